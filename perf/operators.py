@@ -264,7 +264,7 @@ def _plan_plain(s):
     fits = ((ctx + new) <= most * page) & (end <= rows) & ~gone
     need = torch.where(fits, (ctx + new + page - 1) // page - held, 0)
     off = torch.cumsum(need, 0) - need
-    ok = fits & (off + need <= top)
+    ok = fits & ((need == 0) | (off + need <= top))  # one that needs no page goes on
     taken = torch.where(ok, need, 0)
     fresh = (column >= held[:, None]) & (column < (held + taken)[:, None])
     at = top - 1 - (off[:, None] + column - held[:, None])
