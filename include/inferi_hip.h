@@ -251,6 +251,140 @@ IFR_API ifr_status ifr_attention(ifr_ctx *ctx, const ifr_attn_params *params, co
                                  const float *q, const void *key_cache, const void *value_cache, int32_t kv_dtype,
                                  float *xb);
 
+/* ------------------------------------- several requests, a paged cache */
+
+/* A KV cache in pages, for steps that carry rows of several requests (the
+ * reference runs one sequence over one contiguous cache, transformer.rs:85-104).
+ * Row t of page p, KV head h, dim d of the keys is key[p * page_stride +
+ * t * row_stride + h * head_stride + d], in elements; strides of 0 are the
+ * dense [page][row][head][dim].  A row is a contiguous cache as well: page_size
+ * = its length, block_table = {0}.  Row i of request r lies on page
+ * block_table[r * max_pages + i / page_size], at row i % page_size of it.  A
+ * table entry that is no page (>= n_pages; IFR_NO_PAGE by custom) is never
+ * followed: its rows are not written, and attention does not see them.
+ *   dtype        IFR_F16 or IFR_F32
+ *   page_size    a power of two, 16 to 2^30
+ *   head_size    a multiple of 8, at most 128
+ *   max_pages    entries of a request in the table; max_pages * page_size
+ *                at most 2^30
+ *   key, value   16-byte aligned, strides of whole 16 bytes (row and head
+ *                strides at most 2^25 elements); block_table 4-byte aligned
+ * Buffers are the caller's; rows of a request that are not written yet may
+ * hold anything (NaN too). */
+#define IFR_NO_PAGE 0xFFFFFFFFu
+#define IFR_NO_ROW 0xFFFFFFFFu           /* position of a row that is not in the step */
+#define IFR_NO_SLOT 0xFFFFFFFFFFFFFFFFull /* its slot */
+#define IFR_RELEASE 0xFFFFFFFFu          /* new_len of a request whose pages go back */
+typedef struct {
+    void *key, *value;
+    const uint32_t *block_table; /* device, [n_requests][max_pages]; not read by ifr_paged_rope_store */
+    int32_t dtype;
+    uint32_t n_pages, page_size, max_pages, n_kv_heads, head_size;
+    int64_t page_stride, row_stride, head_stride;
+} ifr_paged_cache;
+
+/* A step's bookkeeping on the device: from each request's rows in the cache
+ * (ctx_len) and new rows (new_len), pages from the free list, the block
+ * table's new entries, and for the step's packed rows (request by request, in
+ * order) their positions and slots.
+ *   free_pages[0 .. *free_count) is a stack of page numbers, its top last.
+ *   First the pages of requests with new_len IFR_RELEASE are pushed, in the
+ *   order of requests and of their table rows (entries that are no page are
+ *   left out).  Then the others take theirs from the top, in order: request
+ *   r needs ceil((ctx + new) / page_size) - ceil(ctx / page_size).
+ *   A request is refused, and takes nothing, if ctx + new is more than its
+ *   table row holds or its rows end past n_rows (it then counts for no pages),
+ *   or if it needs pages and it and the requests before it need more than there
+ *   are (one that needs none goes on; later ones get none of what is left).
+ * Out, per request: row_start[r] (n_requests + 1 entries, the last the sum of
+ * all new_len; none above n_rows), kv_len[r] (rows in the cache once the new
+ * ones are stored; 0 if refused or released: its rows attend to nothing),
+ * ctx_len_out[r] (what the next step passes as ctx_len; ctx if refused, 0 if
+ * released), the new table entries, *free_count_out.  Per row, for n_rows
+ * rows: positions[i] and slots[i] = page * page_size + row in page;
+ * IFR_NO_ROW and IFR_NO_SLOT for rows of a refused request and past the last
+ * one.  A slot on an entry that is no page is IFR_NO_SLOT.
+ * ctx_len_out may be ctx_len and free_count_out free_count; no other buffers
+ * may overlap.  A page belongs to one request at a time. */
+typedef struct {
+    uint32_t n_requests, n_rows, n_pages, page_size, max_pages;
+    const uint32_t *ctx_len, *new_len; /* device, [n_requests] */
+    uint32_t *free_pages;              /* device, [n_pages] */
+    const uint32_t *free_count;        /* device, 1 */
+    uint32_t *free_count_out;          /* device, 1 */
+    uint32_t *block_table;             /* device, [n_requests][max_pages] */
+    uint32_t *ctx_len_out;             /* device, [n_requests], or NULL */
+    uint32_t *row_start;               /* device, [n_requests + 1] */
+    uint32_t *kv_len;                  /* device, [n_requests] */
+    uint32_t *positions;               /* device, [n_rows] */
+    uint64_t *slots;                   /* device, [n_rows] */
+} ifr_paged_plan_args;
+IFR_API ifr_status ifr_paged_plan(ifr_ctx *ctx, const ifr_paged_plan_args *args);
+
+/* Rotary embedding of n_rows packed rows, each at its own position, and the
+ * store of their k and v to the cache's slots (one launch; ifr_rope turns one
+ * row at one position).  Row i: q heads at q + i * ld_q, k at k + i * ld_k, v
+ * at v + i * ld_v (f32; the three may be parts of one row of a Q/K/V
+ * product); ld 0 is dense.  Angles are pos * base_freq^(-2j / head_size), formed and
+ * reduced in 64 bits (ifr_rope follows the reference's f32 angles); base_freq
+ * 0 turns nothing.  variant as ifr_rope.  The turned q goes to q_out (q_dtype
+ * IFR_F16 or IFR_F32, ld_q_out); q_out may be q itself if both are f32 with the
+ * same ld.  q and q_out may both be NULL (k and v only).  Values are rounded once, to the
+ * output's or the cache's type.  A row whose position is IFR_NO_ROW is left
+ * out altogether; one whose slot is not in the cache stores nothing, but its
+ * q is turned.  A slot that two rows share ends with one row's values, which
+ * one is not said.  q, k, v 16-byte aligned, ld_q, ld_k, ld_v
+ * multiples of 4, q_out 16-byte aligned with ld_q_out a multiple of 8. */
+typedef struct {
+    uint32_t n_rows, n_heads;
+    int32_t variant;
+    float base_freq;
+    const float *q, *k, *v;
+    int64_t ld_q, ld_k, ld_v;
+    const uint32_t *positions; /* device, [n_rows] */
+    const uint64_t *slots;     /* device, [n_rows] */
+    void *q_out;
+    int32_t q_dtype;
+    int64_t ld_q_out;
+} ifr_paged_rope_args;
+IFR_API ifr_status ifr_paged_rope_store(ifr_ctx *ctx, const ifr_paged_cache *cache, const ifr_paged_rope_args *args);
+
+/* Attention of each request's new rows over its rows of the cache, which hold
+ * the new rows' k and v already: row i of request r (row row_start[r] + i of q
+ * and out, n = row_start[r + 1] - row_start[r] rows) is at position
+ * p = kv_len[r] - n + i and sees the rows j <= p; with window > 0 only those
+ * with j > p - window or j < n_sinks.
+ *   out = softmax_j(scale * q . k_j) . v_j per query head; scale 0 is
+ *   1 / sqrt(head_size); query head h reads KV head h / (n_heads / n_kv_heads).
+ * Rows that see nothing (a refused request's, p < 0, no page) are 0, and so is
+ * a row none of whose scores is above -infinity; rows of no request (from
+ * row_start[n_requests] on) are left as they are.  What a row does not see has no part in
+ * its result, NaN and infinities included (what it sees has: a NaN, or an
+ * infinity in a row of v, as in the formula; an infinity in a row of k may give
+ * NaN).
+ * q and out have q_dtype: IFR_F16 over an F16 cache (products on the matrix
+ * cores, softmax weights rounded to f16, sums in f32) or IFR_F32 over either
+ * (f32 results: q and the weights as two f16 parts each over F16, f32 products
+ * over F32).  ld_q and ld_out in elements, 0 for n_heads * head_size; out may
+ * be q, with the same ld.  max_new and max_kv are the caller's bounds on a request's rows and on
+ * kv_len: they size the launch, and lengths past them are slower, not wrong
+ * (0: n_rows, and what a table row holds).  kv_len is capped at
+ * max_pages * page_size.  One row per request is the decode step; rows
+ * of prompts and decodes mix freely.  q and out 16-byte aligned, ld_q and ld_out multiples
+ * of 8 (BatchedMultiqueryAttention::launch for one row and one contiguous cache,
+ * crates/inferi/src/ops/batched_multiquery_attention.rs:87-110). */
+typedef struct {
+    uint32_t n_requests, n_rows, n_heads;
+    int32_t q_dtype;
+    uint32_t max_new, max_kv, window, n_sinks;
+    float scale;
+    const uint32_t *row_start, *kv_len; /* device, [n_requests + 1], [n_requests] */
+    const void *q;
+    void *out;
+    int64_t ld_q, ld_out;
+} ifr_paged_attn_args;
+IFR_API ifr_status ifr_paged_attention(ifr_ctx *ctx, const ifr_paged_cache *cache, const ifr_paged_attn_args *args);
+
 /* dev_index[0] = index of the largest of v[0..n), lowest index on ties.
  * Replaces the host-side Sampler::sample_argmax
  * (crates/inferi/src/models/sampler.rs:54-56) so the logits never leave

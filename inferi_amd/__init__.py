@@ -66,6 +66,37 @@ class View(C.Structure):
     _fields_ = [("offset", C.c_int64), ("stride", C.c_int64)]
 
 
+NO_PAGE, NO_ROW, NO_SLOT, RELEASE = 0xFFFFFFFF, 0xFFFFFFFF, 0xFFFFFFFFFFFFFFFF, 0xFFFFFFFF
+
+
+class PagedCache(C.Structure):
+    """ifr_paged_cache: a KV cache in pages; strides of 0 are dense."""
+    _fields_ = [(n, C.c_void_p) for n in ("key", "value", "block_table")] + [("dtype", C.c_int32)] + [
+        (n, C.c_uint32) for n in ("n_pages", "page_size", "max_pages", "n_kv_heads", "head_size")] + [
+        (n, C.c_int64) for n in ("page_stride", "row_stride", "head_stride")]
+
+
+class PagedPlan(C.Structure):
+    """ifr_paged_plan_args: a step's requests, the free list and the plan's outputs."""
+    _fields_ = [(n, C.c_uint32) for n in ("n_requests", "n_rows", "n_pages", "page_size", "max_pages")] + [
+        (n, C.c_void_p) for n in ("ctx_len", "new_len", "free_pages", "free_count", "free_count_out", "block_table",
+                                  "ctx_len_out", "row_start", "kv_len", "positions", "slots")]
+
+
+class PagedRope(C.Structure):
+    """ifr_paged_rope_args: a step's packed q, k and v rows, their positions and slots."""
+    _fields_ = [("n_rows", C.c_uint32), ("n_heads", C.c_uint32), ("variant", C.c_int32), ("base_freq", C.c_float)] + [
+        (n, C.c_void_p) for n in ("q", "k", "v")] + [(n, C.c_int64) for n in ("ld_q", "ld_k", "ld_v")] + [
+        (n, C.c_void_p) for n in ("positions", "slots", "q_out")] + [("q_dtype", C.c_int32), ("ld_q_out", C.c_int64)]
+
+
+class PagedAttentionParams(C.Structure):
+    """ifr_paged_attn_args: the step's rows of each request, the window and the caller's bounds."""
+    _fields_ = [("n_requests", C.c_uint32), ("n_rows", C.c_uint32), ("n_heads", C.c_uint32), ("q_dtype", C.c_int32)] + [
+        (n, C.c_uint32) for n in ("max_new", "max_kv", "window", "n_sinks")] + [("scale", C.c_float)] + [
+        (n, C.c_void_p) for n in ("row_start", "kv_len", "q", "out")] + [("ld_q", C.c_int64), ("ld_out", C.c_int64)]
+
+
 # Every symbol include/inferi_hip.h declares, with its ctypes signature.
 _vp, _i32, _u32, _u64, _sz, _f, _cp = C.c_void_p, C.c_int32, C.c_uint32, C.c_uint64, C.c_size_t, C.c_float, C.c_char_p
 SIGNATURES = {
@@ -99,6 +130,9 @@ SIGNATURES = {
     "ifr_rope_view": (_i32, [_vp, _i32, _vp, _vp, View, _u32, _vp, View, _u32]),
     "ifr_silu_view": (_i32, [_vp, _vp, View, _vp, View, _u32]),
     "ifr_attention": (_i32, [_vp, C.POINTER(AttentionParams), _vp, _vp, _vp, _vp, _i32, _vp]),
+    "ifr_paged_plan": (_i32, [_vp, C.POINTER(PagedPlan)]),
+    "ifr_paged_rope_store": (_i32, [_vp, C.POINTER(PagedCache), C.POINTER(PagedRope)]),
+    "ifr_paged_attention": (_i32, [_vp, C.POINTER(PagedCache), C.POINTER(PagedAttentionParams)]),
     "ifr_argmax": (_i32, [_vp, _vp, _u32, _vp]),
     "ifr_sample": (_i32, [_vp, _vp, _vp, _u32, _f, _f, _vp, _vp]),
     "ifr_quantize": (_i32, [_vp, _vp, _vp, _i32, _u64]),
@@ -326,6 +360,15 @@ class LlmContext:
     def silu_view(self, h1, av, h2, bv, n: int) -> None:
         self._check(lib().ifr_silu_view(self.h, _ptr(h1), View(*av), _ptr(h2), View(*bv), n))
 
+    # several requests over a paged cache
+    def paged_plan(self, plan: PagedPlan) -> None:
+        """Request lengths -> pages, block table, row starts, positions and slots of a step."""
+        self._check(lib().ifr_paged_plan(self.h, C.byref(plan)))
+
+    def paged_rope_store(self, cache: PagedCache, rope: PagedRope) -> None:
+        """RoPE of every packed row at its position, k and v to their slots."""
+        self._check(lib().ifr_paged_rope_store(self.h, C.byref(cache), C.byref(rope)))
+
     def argmax(self, v, n: int, out_index) -> None:
         self._check(lib().ifr_argmax(self.h, _ptr(v), n, _ptr(out_index)))
 
@@ -349,6 +392,15 @@ class BatchedMultiqueryAttention:
     def launch(ctxt: LlmContext, params: AttentionParams, params_gpu, q, key_cache, value_cache, kv_dtype: int, xb) -> None:
         ctxt._check(lib().ifr_attention(ctxt.h, C.byref(params), _ptr(params_gpu), _ptr(q), _ptr(key_cache),
                                         _ptr(value_cache), kv_dtype, _ptr(xb)))
+
+
+class PagedAttention:
+    """Attention of each request's new rows over its pages, one row or many per
+    request, with an optional sliding window and first rows that stay visible."""
+
+    @staticmethod
+    def launch(ctxt: LlmContext, cache: PagedCache, params: PagedAttentionParams) -> None:
+        ctxt._check(lib().ifr_paged_attention(ctxt.h, C.byref(cache), C.byref(params)))
 
 
 # ---------------------------------------------------------------- model --

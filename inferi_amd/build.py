@@ -1,12 +1,13 @@
 """Builds the inferi_hip product library in-tree.
 
-Two artefacts, both written next to this file:
+Three artefacts, all written next to this file:
   inferi_kernels.hsaco  gfx950 code object of csrc/kernels.hip
                         (hipcc --genco --offload-arch=gfx950), loaded at run
                         time with hipModuleLoad;
+  inferi_paged.hsaco    the same of csrc/paged.hip (the paged-cache operators);
   libinferi_hip.so      host library with the C ABI of include/inferi_hip.h
-                        (csrc/host.cpp and csrc/gguf.cpp, C++17, links
-                        libamdhip64).
+                        (csrc/host.cpp, csrc/paged.cpp and csrc/gguf.cpp,
+                        C++17, links libamdhip64).
 
 Every HIP compile carries ``-Xclang -target-feature -Xclang -packed-fp32-ops``
 so the compiler never emits packed FP32 instructions.
@@ -24,7 +25,10 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HSACO = os.path.join(HERE, "inferi_kernels.hsaco")
+PAGED_HSACO = os.path.join(HERE, "inferi_paged.hsaco")
 LIB = os.path.join(HERE, "libinferi_hip.so")
+
+HOST_SOURCES = [os.path.join(CSRC, n) for n in ("host.cpp", "paged.cpp", "gguf.cpp")]
 
 HIP_FLAGS = [
     "--genco",
@@ -42,12 +46,16 @@ def _run(cmd: list[str]) -> None:
         raise RuntimeError(f"build step failed ({r.returncode}): {' '.join(cmd)}")
 
 
-def build_kernels(out: str = HSACO) -> str:
+def build_kernels(out: str = HSACO, source: str = "kernels.hip") -> str:
     hipcc = os.path.join(ROCM, "bin", "hipcc")
     tmp = out + ".tmp"
-    _run([hipcc, *HIP_FLAGS, os.path.join(CSRC, "kernels.hip"), "-o", tmp])
+    _run([hipcc, *HIP_FLAGS, os.path.join(CSRC, source), "-o", tmp])
     os.replace(tmp, out)
     return out
+
+
+def build_paged_kernels(out: str = PAGED_HSACO) -> str:
+    return build_kernels(out, "paged.hip")
 
 
 def build_host(out: str = LIB) -> str:
@@ -64,7 +72,7 @@ def build_host(out: str = LIB) -> str:
           os.path.join(CSRC, "noalloc.hip"), "-o", noalloc_o])
     _run([cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall", "-Wextra", "-Wno-unused-result",
           "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__", f"-I{ROCM}/include",
-          os.path.join(CSRC, "host.cpp"), os.path.join(CSRC, "gguf.cpp"), noalloc_o,
+          *HOST_SOURCES, noalloc_o,
           f"-L{ROCM}/lib", "-lamdhip64", f"-Wl,-rpath,{ROCM}/lib", "-o", tmp])
     os.replace(tmp, out)
     return out
@@ -93,17 +101,19 @@ def build_host_asan(out: str = ASAN_LIB) -> str:
         build_host()
     _run([cxx, "-O1", "-g", "-fsanitize=address", "-fno-omit-frame-pointer", "-std=c++17", "-shared", "-fPIC",
           "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__", f"-I{ROCM}/include",
-          os.path.join(CSRC, "host.cpp"), os.path.join(CSRC, "gguf.cpp"), noalloc_o,
+          *HOST_SOURCES, noalloc_o,
           f"-L{ROCM}/lib", "-lamdhip64", f"-Wl,-rpath,{ROCM}/lib", "-o", out])
     return out
 
 
 def build() -> None:
     build_kernels()
+    build_paged_kernels()
     build_host()
 
 
 if __name__ == "__main__":
     build()
     print(HSACO)
+    print(PAGED_HSACO)
     print(LIB)

@@ -1,0 +1,583 @@
+// Attention of several requests' new rows over a paged cache.
+//
+//   out = softmax_j(scale q . k_j) . v_j  over the rows j that the row at
+//   position p sees: j <= p, and under a window w also j > p - w or j < sinks.
+//
+// Work is cut into tiles: the queries q0 .. q0 + QT - 1 of one request times
+// the heads of one KV head (its G query heads, or a sub-group of them), so a
+// K/V row read once serves all of them.  A tile's visible keys are key tiles
+// of the cache (sinks first, then from the window's start to its last
+// query), which up to n_splits workgroups share; with more than one, each
+// leaves a partial (m, l, o) and paged_attn_merge joins them.
+//
+// Scores are kept in base-2 units (scale2 = scale log2 e).  The running
+// reference r of a row (m of the partials) is a value near its maximum so far
+// that the weights 2^(s - r) are taken against; -inf until a score above -inf
+// came, and a row that ends there is 0.
+#pragma once
+#include "../paged_args.h"
+#include "attention.h"
+
+namespace ifr {
+
+typedef float float4v __attribute__((ext_vector_type(4)));
+
+// Operand types: q, cache and output f16; q and output f32 over an f16 cache
+// (q and the softmax weights in two f16 parts each, 22 bits); all f32 (f32
+// matrix products).
+enum PaType : int { PA_H = 0, PA_M = 1, PA_S = 2 };
+
+// A tile of a request's queries, the same for all lanes.
+struct PaTile {
+    uint32_t r, row0;   // request; packed row of the first query
+    uint32_t nq;        // queries
+    int32_t p0, plast;  // positions of the first and last query (p0 may be negative)
+};
+// Its key tiles of KT rows: `ns` from row 0 (sinks), then from tile `lo`; n in all.
+struct PaKeys {
+    uint32_t ns, lo, n;
+};
+template <int KT>
+IFR_DEV PaKeys pa_keys(const PagedAttnArgs &a, const PaTile &t) {
+    PaKeys k = {0, 0, 0};
+    if (t.plast < 0) return k;
+    const uint32_t first = a.window ? (uint32_t)max(t.p0 - (int32_t)a.window + 1, 0) : 0u;
+    k.lo = first / KT;
+    k.ns = min((min(a.sinks, first) + KT - 1) / KT, k.lo);
+    k.n = k.ns + (uint32_t)t.plast / KT + 1 - k.lo;
+    return k;
+}
+// Key tiles of each split: whole multiples shared evenly.
+IFR_DEV uint32_t pa_chunk(const PagedAttnArgs &a, uint32_t n) { return max((n + a.n_splits - 1) / a.n_splits, 1u); }
+
+// Rows and cache length of request r, whatever the buffers hold.
+IFR_DEV void pa_request(const PagedAttnArgs &a, uint32_t r, uint32_t &row0, uint32_t &n, uint32_t &kv) {
+    row0 = min(a.row_start[r], a.n_rows);
+    n = min(max(a.row_start[r + 1], row0), a.n_rows) - row0;
+    kv = min(a.kv_len[r], a.max_pages << a.lp);
+}
+// Queries [q0, q0 + QT) of request r's n rows from row0.
+IFR_DEV PaTile pa_tile(const PagedAttnArgs &a, uint32_t r, uint32_t row0, uint32_t n, uint32_t kv, uint32_t q0) {
+    PaTile t;
+    t.r = r;
+    t.row0 = row0 + q0;
+    t.nq = min(a.QT, n - q0);
+    // a request without rows in the cache (refused) sees nothing
+    t.p0 = kv ? (int32_t)kv - (int32_t)n + (int32_t)q0 : -(1 << 30);
+    t.plast = t.p0 + (int32_t)t.nq - 1;
+    return t;
+}
+// The `at`-th tile, counted from the last, of all requests that the launch
+// serves; false if there are fewer.  64 requests a step, one a lane.
+IFR_DEV bool pa_find(const PagedAttnArgs &a, uint32_t at, uint32_t &r, uint32_t &q0) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t left = at;
+    for (uint32_t top = a.n_requests; top;) {
+        // lane 0 has the last request not yet counted
+        const uint32_t i = top - 1 - lane;
+        uint32_t nt = 0;
+        if (lane < top) {
+            uint32_t row0, n, kv;
+            pa_request(a, i, row0, n, kv);
+            if (n >= a.lo_new && n <= a.hi_new) nt = (n + a.QT - 1) / a.QT;
+        }
+        uint32_t sum = nt;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t u = __shfl_up(sum, d, 64);
+            if (lane >= (uint32_t)d) sum += u;
+        }
+        const uint64_t has = __ballot(sum > left);
+        if (has) {
+            const int src = __ffsll((unsigned long long)has) - 1;
+            const uint32_t s = __shfl(sum, src, 64);
+            r = __builtin_amdgcn_readfirstlane(top - 1 - (uint32_t)src);
+            q0 = __builtin_amdgcn_readfirstlane((s - 1 - left) * a.QT);
+            return true;
+        }
+        left -= __shfl(sum, 63, 64);
+        top -= min(top, 64u);
+    }
+    return false;
+}
+
+// max and sum over the four lanes of a row (lanes n, n + 16, n + 32, n + 48)
+IFR_DEV float pa_max4(float v) {
+    return attn_groups_reduce<128>(v, [](float x, float y) { return fmaxf(x, y); });
+}
+IFR_DEV float pa_sum4(float v) {
+    return attn_groups_reduce<128>(v, [](float x, float y) { return x + y; });
+}
+
+// x in two f16 parts: 22 bits of it (both parts rounded to nearest)
+IFR_DEV void pa_split(float x, _Float16 &hi, _Float16 &lo) {
+    hi = (_Float16)x;
+    lo = (_Float16)(x - (float)hi);
+}
+
+// Whether any half of the words is infinite or NaN, collected over words: the
+// largest |half| so far in each half of acc.
+typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
+IFR_DEV uint32_t pa_odd_acc(uint32_t acc, uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, acc),
+                                                                  __builtin_bit_cast(ushort2v, w & 0x7FFF7FFFu)));
+}
+IFR_DEV bool pa_odd_any(uint32_t acc) { return (acc & 0xFFFFu) >= 0x7C00u || acc >= 0x7C000000u; }
+
+IFR_DEV bool pa_odd(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; } // infinite or NaN
+
+// --------------------------------------------------------- 16-row kernel --
+// One workgroup of four waves per (tile, KV head, sub-group of heads, split):
+// the tile's up to 16 (query, head) rows are one side of every product, and
+// the waves take the split's key tiles of 32 rows in turn.  K and V go from
+// the cache straight into registers in the layout the matrix products read:
+//   S^T = K Q^T   lane (n = lane % 16, g = lane / 16) loads 16 bytes of the rows n
+//                 and 16 + n of the key tile at dims 32c + 8g;
+//   O^T = V^T P^T lane loads dims 8n .. 8n + 7 of the rows 16u + 4g + e (a whole
+//                 row per 16 lanes): the score accumulator holds exactly the
+//                 weights of these rows for query row n, so P^T needs no
+//                 exchange, and V^T's operand for output tile t is element t of
+//                 the eight rows' loads, an 8 x 8 transpose of halves inside
+//                 the lane (output row i of tile t is dim 8i + t).
+// So there is no LDS and no barrier in the loop; the waves' states are joined
+// through LDS once.  Rows whose page is no page read page 0 and are masked.
+constexpr int PAD_WAVES = 4, PAD_KT = 32, PAD_ROWS = 16;
+
+template <int HSP, int T>
+struct PaRegs {
+    static constexpr int KC = T == PA_S ? HSP / 16 : HSP / 32; // 16-byte loads of a K row
+    static constexpr int DV = HSP / 16;                        // dims of a V row per lane
+    uint4 k[2][KC];
+    uint32_t v[8][T == PA_S ? DV : DV / 2];
+};
+
+template <int HSP, int T>
+__device__ void pa_rows16_body(const PagedAttnArgs &a) {
+    constexpr int ES = T == PA_S ? 4 : 2, KC = PaRegs<HSP, T>::KC, DV = HSP / 16;
+    constexpr int OP = HSP + 4;
+    __shared__ __attribute__((aligned(16))) float og[PAD_WAVES][PAD_ROWS][OP];
+    __shared__ float mg[PAD_WAVES][PAD_ROWS], lg[PAD_WAVES][PAD_ROWS];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    uint32_t b = blockIdx.x;
+    const uint32_t kvh = b % a.n_kv;
+    b /= a.n_kv;
+    const uint32_t sub = b % a.n_sub, split = blockIdx.y;
+    b /= a.n_sub;
+    const uint32_t hs = a.hs, heads = min(a.heads_per, a.G - sub * a.heads_per);
+    uint32_t r = b, q0 = 0, row0, nrows, kv;
+    if (a.search && !pa_find(a, b, r, q0)) return;
+    pa_request(a, r, row0, nrows, kv);
+    if (nrows < a.lo_new || nrows > a.hi_new) return;
+    const uint32_t qend = a.search ? q0 + 1 : nrows;
+    const uint32_t *tab = a.table + (size_t)r * a.max_pages;
+    const uint32_t pm = (1u << a.lp) - 1;
+    const uint32_t qi = n / heads, hj = sub * a.heads_per + n % heads; // this lane's row
+    const uint32_t head = kvh * a.G + hj;
+
+    for (; q0 < qend; q0 += a.QT) {
+        const PaTile t = pa_tile(a, r, row0, nrows, kv, q0);
+        const PaKeys keys = pa_keys<PAD_KT>(a, t);
+        const uint32_t C = pa_chunk(a, keys.n), i0 = split * C, i1 = min(i0 + C, keys.n);
+        const bool one = keys.n <= C; // (a tile without keys too: split 0 writes its zeros)
+        if (i0 >= i1 && !(one && split == 0)) continue;
+        const bool row_ok = qi < t.nq;
+        const int32_t qpos = row_ok ? t.p0 + (int32_t)qi : -1;
+        const uint32_t gq = t.row0 + (row_ok ? qi : 0); // packed row
+
+        // q: dims 32c + 8g .. of row n (f32 cache: 16c + 4g ..)
+        half8v qh[T == PA_S ? 1 : KC], ql[T == PA_M ? KC : 1];
+        float4v qf[T == PA_S ? KC : 1];
+        float rs = a.scale2; // of the row's raw scores
+        {
+            const char *qp = (const char *)a.q + ((size_t)gq * a.ld_q + (size_t)head * hs) * (T == PA_H ? 2 : 4);
+            if constexpr (T == PA_H) {
+#pragma unroll
+                for (int c = 0; c < KC; c++) {
+                    const uint32_t d = 32 * c + 8 * g;
+                    const bool ok = row_ok && d < hs;
+                    uint4 x = *(const uint4 *)(qp + 2 * (ok ? d : 0));
+                    if (!ok) x = make_uint4(0, 0, 0, 0);
+                    qh[c] = __builtin_bit_cast(half8v, x);
+                }
+            } else if constexpr (T == PA_M) {
+                // scaled by a power of two that puts the row's largest value in [2^14, 2^15)
+                float x[KC][8], mx = 0.0f;
+#pragma unroll
+                for (int c = 0; c < KC; c++) {
+                    const uint32_t d = 32 * c + 8 * g;
+                    const bool ok = row_ok && d < hs;
+                    const float4 u = *(const float4 *)(qp + 4 * (ok ? d : 0)), w = *(const float4 *)(qp + 4 * (ok ? d : 0) + 16);
+                    const float y[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        x[c][e] = ok ? y[e] : 0.0f;
+                        mx = fmaxf(mx, fabsf(x[c][e]));
+                    }
+                }
+                mx = pa_max4(mx);
+                const int ex = mx > 0.0f && !pa_odd(mx) ? min(14 - ilogbf(mx), 100) : 0;
+                rs = ldexpf(rs, -ex);
+#pragma unroll
+                for (int c = 0; c < KC; c++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        _Float16 hi, lo;
+                        pa_split(ldexpf(x[c][e], ex), hi, lo);
+                        qh[c][e] = hi;
+                        ql[c][e] = lo;
+                    }
+            } else {
+#pragma unroll
+                for (int c = 0; c < KC; c++) {
+                    const uint32_t d = 16 * c + 4 * g;
+                    const bool ok = row_ok && d < hs;
+                    const float4 x = *(const float4 *)(qp + 4 * (ok ? d : 0));
+                    qf[c] = ok ? float4v{x.x, x.y, x.z, x.w} : float4v{0, 0, 0, 0};
+                }
+            }
+        }
+
+        float4v o[DV];
+#pragma unroll
+        for (int d = 0; d < DV; d++) o[d] = float4v{0, 0, 0, 0};
+        float m = -INFINITY, l = 0.0f;
+
+        auto tile_of = [&](uint32_t i) { return i < keys.ns ? i : keys.lo + i - keys.ns; };
+        // page of the 16 rows from 16 * b16
+        auto page_of = [&](uint32_t b16) { return tab[min(b16 >> (a.lp - 4), a.max_pages - 1)]; };
+        PaRegs<HSP, T> x;
+        const uint32_t dk = T == PA_S ? 4 * g : 8 * g, dv = DV * n;
+        auto base_of = [&](const void *p, uint32_t page, uint32_t row) {
+            return (const char *)p + ((int64_t)(page < a.n_pages ? page : 0u) * a.page_stride +
+                                      (int64_t)(row & pm) * a.row_stride + (int64_t)kvh * a.head_stride) * ES;
+        };
+        auto load_k = [&](uint32_t kt, uint32_t pg0, uint32_t pg1) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const char *p = base_of(a.key, u ? pg1 : pg0, kt * PAD_KT + 16 * u);
+                const uint32_t off = n * (uint32_t)a.row_stride;
+#pragma unroll
+                for (int c = 0; c < KC; c++) {
+                    const uint32_t d = (T == PA_S ? 16 : 32) * c + dk;
+                    x.k[u][c] = *(const uint4 *)(p + (size_t)(off + (HSP == 128 && hs == 128 ? d : min(d, hs - (T == PA_S ? 4 : 8)))) * ES);
+                }
+            }
+        };
+        auto load_v = [&](uint32_t kt, uint32_t pg0, uint32_t pg1) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const char *p = base_of(a.value, u ? pg1 : pg0, kt * PAD_KT + 16 * u);
+                const uint32_t d = min(dv, hs - DV);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const char *s = p + (size_t)((4 * g + e) * (uint32_t)a.row_stride + d) * ES;
+                    uint32_t *w = x.v[4 * u + e];
+                    constexpr int W = sizeof(x.v[0]) / 4; // 2, 4 or 8 words
+                    if constexpr (W == 2) {
+                        const uint2 y = *(const uint2 *)s;
+                        w[0] = y.x; w[1] = y.y;
+                    } else {
+#pragma unroll
+                        for (int z = 0; z < W; z += 4) {
+                            const uint4 y = *(const uint4 *)(s + 4 * z);
+                            w[z] = y.x; w[z + 1] = y.y; w[z + 2] = y.z; w[z + 3] = y.w;
+                        }
+                    }
+                }
+            }
+        };
+
+        uint32_t i = i0 + wave;
+        if (i < i1) {
+            uint32_t kt = tile_of(i), pg0 = page_of(2 * kt), pg1 = page_of(2 * kt + 1);
+            load_k(kt, pg0, pg1);
+            load_v(kt, pg0, pg1);
+            uint32_t nx = min(i + PAD_WAVES, i1 - 1), kn = tile_of(nx), pn0 = page_of(2 * kn), pn1 = page_of(2 * kn + 1);
+            for (; i < i1; i += PAD_WAVES) {
+                const uint32_t k0 = kt * PAD_KT;
+                if (hs != HSP) { // (uniform) dims past the head size: zero, as q's are (0 x inf is not)
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int c = 0; c < KC; c++)
+                            if ((T == PA_S ? 16 : 32) * c + dk >= hs) x.k[u][c] = make_uint4(0, 0, 0, 0);
+                }
+                float4v s[2];
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    s[u] = float4v{0, 0, 0, 0};
+#pragma unroll
+                    for (int c = 0; c < KC; c++) {
+                        if constexpr (T == PA_S) {
+                            const float4v kf = __builtin_bit_cast(float4v, x.k[u][c]);
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[c][e], s[u], 0, 0, 0);
+                        } else {
+                            const half8v kh = __builtin_bit_cast(half8v, x.k[u][c]);
+                            s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[c], s[u], 0, 0, 0);
+                            if constexpr (T == PA_M)
+                                s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[c], s[u], 0, 0, 0);
+                        }
+                    }
+                }
+                const bool bad0 = pg0 >= a.n_pages, bad1 = pg1 >= a.n_pages;
+                // the next tile's K (past the last: the last again, unused)
+                load_k(kn, pn0, pn1);
+                // keys that not every row of the tile sees
+                const bool partly = (int32_t)(k0 + PAD_KT - 1) > t.p0 ||
+                                    (a.window && (int64_t)k0 <= (int64_t)t.plast - a.window) || bad0 || bad1;
+                bool fix = false;
+#pragma unroll
+                for (int u = 0; u < 2; u++) s[u] *= rs;
+                if (partly) {
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int32_t key = (int32_t)(k0 + 16 * u + 4 * g + e);
+                            const bool page_ok = !(u ? bad1 : bad0);
+                            const bool see = page_ok && key <= qpos &&
+                                             (!a.window || key > qpos - (int32_t)a.window || key < (int32_t)a.sinks);
+                            s[u][e] = see ? s[u][e] : -INFINITY;
+                            // a key that no row sees has no part in the sums, whatever it holds; one that
+                            // some rows see and others do not must be finite to be multiplied by 0
+                            const bool any = page_ok && key <= t.plast &&
+                                             (!a.window || key > t.p0 - (int32_t)a.window || key < (int32_t)a.sinks);
+#pragma unroll
+                            for (int z = 0; z < (int)(sizeof(x.v[0]) / 4); z++) {
+                                uint32_t &w = x.v[4 * u + e][z];
+                                w = any ? w : 0u;
+                                if constexpr (T == PA_S) fix |= (w & 0x7F800000u) == 0x7F800000u;
+                            }
+                        }
+                }
+                if constexpr (T != PA_S) {
+                    // the two parts of a weight would multiply an infinity that all rows see to NaN: every tile then
+                    if (partly || T == PA_M) {
+                        uint32_t acc = 0;
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+#pragma unroll
+                            for (int z = 0; z < (int)(sizeof(x.v[0]) / 4); z++) acc = pa_odd_acc(acc, x.v[j][z]);
+                        fix = pa_odd_any(acc);
+                    }
+                }
+                float mt = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mt = fmaxf(mt, s[u][e]);
+                mt = pa_max4(mt);
+                // the reference moves only where a row's maximum passes it by more than 8: the weights stay
+                // below 2^8 (f16 holds them as well as those below 1) and most tiles rescale nothing
+                if (__ballot(mt > m + 8.0f)) {
+                    const float mn = fmaxf(m, mt), al = mn == -INFINITY ? 0.0f : softmax_exp2(m - mn);
+                    m = mn;
+                    l *= al;
+#pragma unroll
+                    for (int d = 0; d < DV; d++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[d][e] *= al;
+                }
+                const float mr = m == -INFINITY ? 0.0f : m;
+                float p[8];
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        p[4 * u + e] = softmax_exp2(s[u][e] - mr);
+                        l += p[4 * u + e];
+                    }
+                if (__ballot(fix)) {
+                    // infinities or NaN in rows of V that not all rows of the tile see: their products are
+                    // formed one by one for the rows that do, and they are 0 in the matrix products
+                    for (int j = 0; j < 8; j++)
+                        for (uint32_t gg = 0; gg < 4; gg++) {
+                            const uint32_t kr = k0 + 16 * (j >> 2) + 4 * gg + (j & 3);
+                            float pj = 0.0f;
+#pragma unroll
+                            for (int z = 0; z < 8; z++) pj = z == j ? p[z] : pj;
+                            pj = __shfl(pj, (int)(n + 16 * gg), 64);
+                            const int32_t key = (int32_t)kr;
+                            const bool see = !((j >> 2) ? bad1 : bad0) && key <= qpos &&
+                                             (!a.window || key > qpos - (int32_t)a.window || key < (int32_t)a.sinks);
+                            if (!see) continue;
+                            const char *vp = base_of(a.value, (j >> 2) ? pg1 : pg0, kr);
+#pragma unroll
+                            for (int d = 0; d < DV; d++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    const uint32_t dim = DV * (4 * g + e) + d;
+                                    if (dim >= hs) continue;
+                                    const float vv = T == PA_S ? ((const float *)vp)[dim] : (float)((const _Float16 *)vp)[dim];
+                                    if (pa_odd(vv)) o[d][e] += pj * vv;
+                                }
+                        }
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+#pragma unroll
+                        for (int z = 0; z < (int)(sizeof(x.v[0]) / 4); z++) {
+                            uint32_t &w = x.v[j][z];
+                            if constexpr (T == PA_S) {
+                                if ((w & 0x7F800000u) == 0x7F800000u) w = 0;
+                            } else {
+                                if ((w & 0x7C00u) == 0x7C00u) w &= 0xFFFF0000u;
+                                if ((w & 0x7C000000u) == 0x7C000000u) w &= 0xFFFFu;
+                            }
+                        }
+                }
+                if constexpr (T == PA_S) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+#pragma unroll
+                        for (int d = 0; d < DV; d++)
+                            o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.v[j][d]), p[j], o[d], 0, 0, 0);
+                } else {
+                    half8v ph, pl;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        _Float16 hi, lo;
+                        pa_split(p[j], hi, lo);
+                        ph[j] = hi;
+                        pl[j] = lo;
+                    }
+#pragma unroll
+                    for (int d = 0; d < DV; d++) {
+                        // halves d of the eight rows' loads: the low or high half of word d / 2
+                        uint4 w;
+                        const uint32_t sel = (d & 1) ? 0x07060302u : 0x05040100u;
+                        w.x = __builtin_amdgcn_perm(x.v[1][d / 2], x.v[0][d / 2], sel);
+                        w.y = __builtin_amdgcn_perm(x.v[3][d / 2], x.v[2][d / 2], sel);
+                        w.z = __builtin_amdgcn_perm(x.v[5][d / 2], x.v[4][d / 2], sel);
+                        w.w = __builtin_amdgcn_perm(x.v[7][d / 2], x.v[6][d / 2], sel);
+                        const half8v vt = __builtin_bit_cast(half8v, w);
+                        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, ph, o[d], 0, 0, 0);
+                        if constexpr (T == PA_M) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, pl, o[d], 0, 0, 0);
+                    }
+                }
+                kt = kn;
+                load_v(kt, pn0, pn1);
+                pg0 = pn0;
+                pg1 = pn1;
+                nx = min(i + 2 * PAD_WAVES, i1 - 1);
+                kn = tile_of(nx);
+                pn0 = page_of(2 * kn);
+                pn1 = page_of(2 * kn + 1);
+            }
+        }
+
+        // the waves' states through LDS
+        l = pa_sum4(l);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int d = 0; d < DV; d++) og[wave][n][DV * (4 * g + e) + d] = o[d][e];
+        if (g == 0) {
+            mg[wave][n] = m;
+            lg[wave][n] = l;
+        }
+        __syncthreads();
+        const uint32_t rows = t.nq * heads, quads = hs / 4;
+        for (uint32_t it = tid; it < rows * quads; it += 64 * PAD_WAVES) {
+            const uint32_t rr = it / quads, d = 4 * (it % quads);
+            float M = -INFINITY, L = 0.0f, O[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < PAD_WAVES; w++) M = fmaxf(M, mg[w][rr]);
+            const float mr = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+            for (int w = 0; w < PAD_WAVES; w++) {
+                const float wt = softmax_exp2(mg[w][rr] - mr);
+                const float4 y = *(const float4 *)&og[w][rr][d];
+                L = fmaf(lg[w][rr], wt, L);
+                O[0] = fmaf(y.x, wt, O[0]);
+                O[1] = fmaf(y.y, wt, O[1]);
+                O[2] = fmaf(y.z, wt, O[2]);
+                O[3] = fmaf(y.w, wt, O[3]);
+            }
+            const size_t orow = t.row0 + rr / heads, ohead = kvh * a.G + sub * a.heads_per + rr % heads;
+            if (one) {
+                const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+                char *dst = (char *)a.out + (orow * a.ld_out + ohead * hs + d) * (T == PA_H ? 2 : 4);
+                // a row that saw nothing has O = 0
+                const float y[4] = {O[0] * inv, O[1] * inv, O[2] * inv, O[3] * inv};
+                if constexpr (T == PA_H)
+                    *(uint2 *)dst = make_uint2((uint32_t)f32_to_f16(y[0]) | (uint32_t)f32_to_f16(y[1]) << 16,
+                                               (uint32_t)f32_to_f16(y[2]) | (uint32_t)f32_to_f16(y[3]) << 16);
+                else *(float4 *)dst = make_float4(y[0], y[1], y[2], y[3]);
+            } else {
+                const size_t at = (orow * ((size_t)a.n_kv * a.G) + ohead) * a.n_splits + split;
+                *(float4 *)(a.part_o + at * hs + d) = make_float4(O[0], O[1], O[2], O[3]);
+                if (d == 0) *(float2 *)(a.part_ml + at * 2) = make_float2(M, L);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Joins the splits of tiles of the kernel above (KT 32) or of the tile kernel
+// (KT 64): grid as its x.  A wave takes a row of the tile at a time, a lane
+// the dims 2 lane, 2 lane + 1 (64 dims: one).  Only splits that the tile has are
+// read; a tile of one split is written already.
+template <int HSP, int T, int KT>
+__device__ void pa_merge_body(const PagedAttnArgs &a) {
+    constexpr int E = HSP / 64;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint32_t b = blockIdx.x;
+    const uint32_t kvh = b % a.n_kv;
+    b /= a.n_kv;
+    const uint32_t sub = b % a.n_sub;
+    b /= a.n_sub;
+    const uint32_t hs = a.hs, heads = min(a.heads_per, a.G - sub * a.heads_per);
+    uint32_t r = b, q0 = 0, row0, nrows, kv;
+    if (a.search && !pa_find(a, b, r, q0)) return;
+    pa_request(a, r, row0, nrows, kv);
+    if (nrows < a.lo_new || nrows > a.hi_new) return;
+    const uint32_t qend = a.search ? q0 + 1 : nrows;
+    for (; q0 < qend; q0 += a.QT) {
+        const PaTile t = pa_tile(a, r, row0, nrows, kv, q0);
+        const uint32_t n = pa_keys<KT>(a, t).n, C = pa_chunk(a, n);
+        if (n <= C) continue;
+        const uint32_t S = (n + C - 1) / C;
+        for (uint32_t rr = wave; rr < t.nq * heads; rr += 4) {
+            const size_t orow = t.row0 + rr / heads, ohead = kvh * a.G + sub * a.heads_per + rr % heads;
+            const size_t at = (orow * ((size_t)a.n_kv * a.G) + ohead) * a.n_splits;
+            // the splits' references one a lane, then their weights
+            float M = -INFINITY;
+            for (uint32_t s = lane; s < S; s += 64) M = fmaxf(M, a.part_ml[(at + s) * 2]);
+            M = wave_max(M);
+            const float mr = M == -INFINITY ? 0.0f : M;
+            float L = 0.0f;
+            for (uint32_t s = lane; s < S; s += 64)
+                L = fmaf(a.part_ml[(at + s) * 2 + 1], softmax_exp2(a.part_ml[(at + s) * 2] - mr), L);
+            L = wave_sum(L);
+            const uint32_t d = E * lane;
+            const bool in = d < hs;
+            float O[E] = {};
+            const float *po = a.part_o + at * hs + (in ? d : 0);
+#pragma unroll 8
+            for (uint32_t s = 0; s < S; s++) {
+                const float w = softmax_exp2(a.part_ml[(at + s) * 2] - mr);
+                if constexpr (E == 2) {
+                    const float2 y = *(const float2 *)(po + (size_t)s * hs);
+                    O[0] = fmaf(y.x, w, O[0]);
+                    O[1] = fmaf(y.y, w, O[1]);
+                } else {
+                    O[0] = fmaf(po[(size_t)s * hs], w, O[0]);
+                }
+            }
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            if (in) {
+                const size_t off = orow * a.ld_out + ohead * hs + d;
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    if constexpr (T == PA_H) ((uint16_t *)a.out)[off + e] = f32_to_f16(O[e] * inv);
+                    else ((float *)a.out)[off + e] = O[e] * inv;
+                }
+            }
+        }
+    }
+}
+
+} // namespace ifr

@@ -1,0 +1,252 @@
+// Host side of the paged-cache operators (include/inferi_hip.h "several
+// requests, a paged cache"): the checks of arguments, the launch shapes and
+// the splits of the attention over the sequence.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <string>
+
+#include "ctx.h"
+#include "paged_args.h"
+
+using namespace ifr;
+
+namespace {
+
+constexpr uint32_t MAX_CONTEXT = 1u << 30;          // max_pages * page_size, as max_pos
+constexpr uint64_t PART_BYTES_MAX = 512ull << 20;   // partials of one attention call
+
+uint32_t log2_of(uint32_t v) { return 31u - (uint32_t)__builtin_clz(v); }
+bool pow2(uint32_t v) { return v && !(v & (v - 1)); }
+
+// Makes the context's device current for a call that may allocate or launch,
+// and the caller's again at its end.
+struct DeviceGuard {
+    int before = -1;
+    explicit DeviceGuard(int device) {
+        int now = 0;
+        if (hipGetDevice(&now) == hipSuccess && now != device && hipSetDevice(device) == hipSuccess) before = now;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) hipSetDevice(before);
+    }
+};
+
+ifr_status check_pages(ifr_ctx *c, const char *who, uint32_t page_size, uint32_t n_pages, uint32_t max_pages) {
+    if (!pow2(page_size) || page_size < 16 || page_size > MAX_CONTEXT)
+        return c->fail(IFR_EINVAL, "%s: page_size %u (a power of two from 16)", who, page_size);
+    if (!n_pages || n_pages == IFR_NO_PAGE) return c->fail(IFR_EINVAL, "%s: n_pages %u", who, n_pages);
+    if (!max_pages || (uint64_t)max_pages * page_size > MAX_CONTEXT)
+        return c->fail(IFR_EINVAL, "%s: max_pages %u of %u rows (at most 2^30 rows)", who, max_pages, page_size);
+    return IFR_OK;
+}
+
+// The cache's arguments, with the dense strides filled in.
+ifr_status check_cache(ifr_ctx *c, const char *who, ifr_paged_cache &k) {
+    if (!k.key || !k.value) return c->fail(IFR_EINVAL, "%s: null cache", who);
+    if (k.dtype != IFR_F16 && k.dtype != IFR_F32) return c->fail(IFR_EINVAL, "%s: cache dtype F16 or F32", who);
+    if (ifr_status st = check_pages(c, who, k.page_size, k.n_pages, k.max_pages)) return st;
+    if (!k.head_size || k.head_size % 8 || k.head_size > 128)
+        return c->fail(IFR_EUNSUPPORTED, "%s: head_size %u (a multiple of 8, at most 128)", who, k.head_size);
+    if (!k.n_kv_heads || k.n_kv_heads > 65535) return c->fail(IFR_EINVAL, "%s: n_kv_heads %u", who, k.n_kv_heads);
+    const int64_t unit = k.dtype == IFR_F16 ? 8 : 4, most = 1 << 25;
+    if (!k.head_stride) k.head_stride = k.head_size;
+    if (!k.row_stride) k.row_stride = (int64_t)k.n_kv_heads * k.head_size;
+    if (!k.page_stride) k.page_stride = (int64_t)k.page_size * k.row_stride;
+    if (k.head_stride < 0 || k.row_stride < 0 || k.page_stride < 0 || k.head_stride % unit || k.row_stride % unit ||
+        k.page_stride % unit || k.row_stride > most || k.page_stride > (1ll << 56) / std::max<int64_t>(k.n_pages, 1) ||
+        k.head_stride > (1ll << 56) / k.n_kv_heads)
+        return c->fail(IFR_EINVAL, "%s: cache strides (whole 16 bytes, rows at most 2^25 elements apart)", who);
+    if ((uintptr_t)k.key % 16 || (uintptr_t)k.value % 16) return c->fail(IFR_EINVAL, "%s: cache not 16-byte aligned", who);
+    return IFR_OK;
+}
+
+bool bad_ld(int64_t ld, int64_t least, int64_t unit) { return ld < least || ld % unit || ld > (1ll << 40); }
+
+} // namespace
+
+extern "C" {
+
+IFR_API ifr_status ifr_paged_plan(ifr_ctx *c, const ifr_paged_plan_args *p) {
+    if (!c) return IFR_EINVAL;
+    if (!p) return c->fail(IFR_EINVAL, "paged_plan: null arguments");
+    if (ifr_status st = check_pages(c, "paged_plan", p->page_size, p->n_pages, p->max_pages)) return st;
+    if (!p->free_count || !p->free_count_out || !p->free_pages || !p->row_start)
+        return c->fail(IFR_EINVAL, "paged_plan: null pointer");
+    if (p->n_requests && (!p->ctx_len || !p->new_len || !p->block_table || !p->kv_len))
+        return c->fail(IFR_EINVAL, "paged_plan: null pointer");
+    if (p->n_rows && (!p->positions || !p->slots)) return c->fail(IFR_EINVAL, "paged_plan: null pointer");
+    if (p->n_rows > MAX_CONTEXT || p->n_requests > MAX_CONTEXT)
+        return c->fail(IFR_EINVAL, "paged_plan: %u rows of %u requests", p->n_rows, p->n_requests);
+    DeviceGuard dev(c->device);
+    PagedPlanArgs a{};
+    a.ctx_len = p->ctx_len;
+    a.new_len = p->new_len;
+    a.free_pages = p->free_pages;
+    a.free_count = p->free_count;
+    a.free_count_out = p->free_count_out;
+    a.table = p->block_table;
+    a.ctx_len_out = p->ctx_len_out;
+    a.row_start = p->row_start;
+    a.kv_len = p->kv_len;
+    a.positions = p->positions;
+    a.slots = p->slots;
+    a.n_requests = p->n_requests;
+    a.n_rows = p->n_rows;
+    a.n_pages = p->n_pages;
+    a.lp = log2_of(p->page_size);
+    a.max_pages = p->max_pages;
+    a.rows_here = p->n_rows <= 2048 || !p->n_requests;
+    const uint32_t threads = p->n_requests <= 256 && p->n_rows <= 256 ? 256 : PG_PLAN_THREADS;
+    ifr_status st = c->launch("paged_plan_k", dim3(1), dim3(threads), 0, a);
+    if (st || a.rows_here) return st;
+    return c->launch("paged_rows_k", dim3((p->n_rows + 511) / 512), dim3(256), 0, a);
+}
+
+IFR_API ifr_status ifr_paged_rope_store(ifr_ctx *c, const ifr_paged_cache *cache, const ifr_paged_rope_args *p) {
+    if (!c) return IFR_EINVAL;
+    if (!cache || !p) return c->fail(IFR_EINVAL, "paged_rope_store: null arguments");
+    ifr_paged_cache k = *cache;
+    k.max_pages = 1; // the table is not read
+    if (ifr_status st = check_cache(c, "paged_rope_store", k)) return st;
+    if (!p->n_rows) return IFR_OK;
+    const uint32_t hs = k.head_size;
+    if (p->variant != IFR_ROPE_ORIGINAL && p->variant != IFR_ROPE_NEOX)
+        return c->fail(IFR_EINVAL, "paged_rope_store: bad variant");
+    if (!(p->base_freq >= 0.0f) || std::isinf(p->base_freq))
+        return c->fail(IFR_EINVAL, "paged_rope_store: base_freq (0, or positive and finite)");
+    if (!p->k || !p->v || !p->positions || !p->slots) return c->fail(IFR_EINVAL, "paged_rope_store: null pointer");
+    if (!p->q != !p->q_out) return c->fail(IFR_EINVAL, "paged_rope_store: q and q_out, or neither");
+    if (p->q && (!p->n_heads || p->n_heads > 65535)) return c->fail(IFR_EINVAL, "paged_rope_store: n_heads %u", p->n_heads);
+    if (p->q && p->q_dtype != IFR_F16 && p->q_dtype != IFR_F32)
+        return c->fail(IFR_EINVAL, "paged_rope_store: q_dtype F16 or F32");
+    if (p->n_rows > MAX_CONTEXT) return c->fail(IFR_EINVAL, "paged_rope_store: n_rows %u", p->n_rows);
+    const int64_t qd = (int64_t)p->n_heads * hs, kd = (int64_t)k.n_kv_heads * hs;
+    PagedRopeArgs a{};
+    a.ld_q = p->ld_q ? p->ld_q : qd;
+    a.ld_k = p->ld_k ? p->ld_k : kd;
+    a.ld_v = p->ld_v ? p->ld_v : kd;
+    a.ld_q_out = p->ld_q_out ? p->ld_q_out : qd;
+    if ((p->q && (bad_ld(a.ld_q, qd, 4) || bad_ld(a.ld_q_out, qd, 8))) || bad_ld(a.ld_k, kd, 4) || bad_ld(a.ld_v, kd, 4))
+        return c->fail(IFR_EINVAL, "paged_rope_store: leading dimensions");
+    if ((uintptr_t)p->q % 16 || (uintptr_t)p->k % 16 || (uintptr_t)p->v % 16 || (uintptr_t)p->q_out % 16)
+        return c->fail(IFR_EINVAL, "paged_rope_store: rows must be 16-byte aligned");
+    if (p->q && (const void *)p->q == p->q_out && (p->q_dtype != IFR_F32 || a.ld_q != a.ld_q_out))
+        return c->fail(IFR_EINVAL, "paged_rope_store: q_out may be q only in f32 with its ld");
+    a.q = p->q;
+    a.k = p->k;
+    a.v = p->v;
+    a.positions = p->positions;
+    a.slots = p->slots;
+    a.q_out = p->q_out;
+    a.key = k.key;
+    a.value = k.value;
+    a.page_stride = k.page_stride;
+    a.row_stride = k.row_stride;
+    a.head_stride = k.head_stride;
+    a.turn = p->base_freq > 0.0f;
+    a.log2_base = a.turn ? std::log2((double)p->base_freq) : 0.0;
+    a.n_rows = p->n_rows;
+    a.n_heads = p->n_heads;
+    a.n_kv = k.n_kv_heads;
+    a.hs = hs;
+    a.n_pages = k.n_pages;
+    a.lp = log2_of(k.page_size);
+    a.neox = p->variant == IFR_ROPE_NEOX;
+    a.q_f16 = p->q_dtype == IFR_F16;
+    a.kv_f16 = k.dtype == IFR_F16;
+    a.rows_per = p->n_rows >= 4 * (uint32_t)c->n_cu ? 4 : 1;
+    const uint32_t items = ((p->q ? p->n_heads : 0) + 2 * k.n_kv_heads) * (hs / 8);
+    a.parts = a.rows_per > 1 ? 1 : std::max(1u, std::min((items + PG_ROPE_THREADS - 1) / PG_ROPE_THREADS,
+                                                         (uint32_t)c->n_cu * 2 / p->n_rows));
+    DeviceGuard dev(c->device);
+    return c->launch("paged_rope_k", dim3((p->n_rows + a.rows_per - 1) / a.rows_per, a.parts), dim3(PG_ROPE_THREADS), 0, a);
+}
+
+IFR_API ifr_status ifr_paged_attention(ifr_ctx *c, const ifr_paged_cache *cache, const ifr_paged_attn_args *p) {
+    if (!c) return IFR_EINVAL;
+    if (!cache || !p) return c->fail(IFR_EINVAL, "paged_attention: null arguments");
+    ifr_paged_cache k = *cache;
+    if (ifr_status st = check_cache(c, "paged_attention", k)) return st;
+    if (!p->n_requests || !p->n_rows) return IFR_OK;
+    const uint32_t hs = k.head_size;
+    if (!k.block_table || !p->row_start || !p->kv_len || !p->q || !p->out)
+        return c->fail(IFR_EINVAL, "paged_attention: null pointer");
+    if (!p->n_heads || p->n_heads > 65535 || p->n_heads % k.n_kv_heads)
+        return c->fail(IFR_EINVAL, "paged_attention: %u heads over %u KV heads", p->n_heads, k.n_kv_heads);
+    if (p->q_dtype != IFR_F16 && p->q_dtype != IFR_F32)
+        return c->fail(IFR_EINVAL, "paged_attention: q_dtype F16 or F32");
+    if (p->q_dtype == IFR_F16 && k.dtype == IFR_F32)
+        return c->fail(IFR_EUNSUPPORTED, "paged_attention: f16 queries over an f32 cache");
+    if (p->n_rows > MAX_CONTEXT || p->n_requests > MAX_CONTEXT)
+        return c->fail(IFR_EINVAL, "paged_attention: %u rows of %u requests", p->n_rows, p->n_requests);
+    if (!std::isfinite(p->scale) || p->scale < 0.0f) return c->fail(IFR_EINVAL, "paged_attention: scale (0, or positive)");
+    const int64_t qd = (int64_t)p->n_heads * hs;
+    PagedAttnArgs a{};
+    a.ld_q = p->ld_q ? p->ld_q : qd;
+    a.ld_out = p->ld_out ? p->ld_out : qd;
+    if (bad_ld(a.ld_q, qd, 8) || bad_ld(a.ld_out, qd, 8)) return c->fail(IFR_EINVAL, "paged_attention: ld_q, ld_out");
+    if ((uintptr_t)p->q % 16 || (uintptr_t)p->out % 16)
+        return c->fail(IFR_EINVAL, "paged_attention: q and out must be 16-byte aligned");
+    if (p->q == p->out && a.ld_q != a.ld_out) return c->fail(IFR_EINVAL, "paged_attention: out may be q only with its ld");
+    const uint32_t cap = k.max_pages * k.page_size;
+    a.q = p->q;
+    a.out = p->out;
+    a.key = k.key;
+    a.value = k.value;
+    a.table = k.block_table;
+    a.row_start = p->row_start;
+    a.kv_len = p->kv_len;
+    a.page_stride = k.page_stride;
+    a.row_stride = k.row_stride;
+    a.head_stride = k.head_stride;
+    a.n_pages = k.n_pages;
+    a.lp = log2_of(k.page_size);
+    a.max_pages = k.max_pages;
+    a.n_kv = k.n_kv_heads;
+    a.hs = hs;
+    a.G = p->n_heads / k.n_kv_heads;
+    a.n_requests = p->n_requests;
+    a.n_rows = p->n_rows;
+    a.window = p->window >= cap ? 0 : p->window;
+    a.sinks = a.window ? std::min(p->n_sinks, cap) : 0;
+    const float scale = p->scale > 0.0f ? p->scale : 1.0f / std::sqrt((float)hs);
+    a.scale2 = scale * 1.44269504088896341f;
+    const char *type = p->q_dtype == IFR_F16 ? "f16" : k.dtype == IFR_F16 ? "mixed" : "f32";
+    const uint32_t hsp = hs <= 64 ? 64 : 128;
+    const uint32_t max_new = p->max_new ? std::min(p->max_new, p->n_rows) : p->n_rows;
+    const uint32_t max_kv = p->max_kv ? std::min(p->max_kv, cap) : cap;
+
+    // 16 (query, head) rows a tile; a group of more heads is cut into sub-groups of 16
+    a.heads_per = std::min(a.G, 16u);
+    a.n_sub = (a.G + 15) / 16;
+    a.QT = std::max(16 / a.G, 1u);
+    a.lo_new = 1;
+    a.hi_new = 0xFFFFFFFFu;
+    a.search = max_new > a.QT;
+    const uint64_t tiles = a.search ? p->n_rows / a.QT + std::min(p->n_requests, p->n_rows) : p->n_requests;
+    const uint64_t base = tiles * a.n_sub * a.n_kv;
+    if (base >= (1u << 23)) return c->fail(IFR_EUNSUPPORTED, "paged_attention: %llu workgroups", (unsigned long long)base);
+    uint64_t keys = max_kv; // rows that a tile reads, at most
+    if (a.window) keys = std::min<uint64_t>(keys, (uint64_t)a.window + a.sinks + a.QT + 64);
+    const uint64_t key_tiles = (keys + 31) / 32;
+    uint64_t splits = (1024 + base - 1) / base;
+    splits = std::max<uint64_t>(1, std::min(splits, (key_tiles + 7) / 8));
+    const uint64_t row_bytes = (uint64_t)p->n_rows * p->n_heads * (hs + 2) * 4;
+    splits = std::max<uint64_t>(1, std::min(splits, PART_BYTES_MAX / row_bytes));
+    a.n_splits = (uint32_t)splits;
+    DeviceGuard dev(c->device);
+    if (splits > 1) {
+        if (ifr_status st = c->ensure_scratch(row_bytes * splits)) return st;
+        a.part_o = (float *)c->scratch;
+        a.part_ml = a.part_o + (uint64_t)p->n_rows * p->n_heads * splits * hs;
+    }
+    char name[64];
+    snprintf(name, sizeof name, "paged_rows16_%s_h%u", type, hsp);
+    ifr_status st = c->launch(name, dim3((uint32_t)base, a.n_splits), dim3(256), 0, a);
+    if (st || splits == 1) return st;
+    snprintf(name, sizeof name, "paged_merge32_%s_h%u", type, hsp);
+    return c->launch(name, dim3((uint32_t)base), dim3(256), 0, a);
+}
+
+} // extern "C"
