@@ -202,6 +202,12 @@ IFR_DEV float rope_theta_f32(float base, float head_dim, float hs) {
     return (float)pow((double)base, (double)(-head_dim / hs));
 }
 
+// x with its bits 2 and 3 exchanged
+IFR_DEV uint32_t swap23(uint32_t x) {
+    const uint32_t t = ((x >> 2) ^ (x >> 3)) & 1u;
+    return x ^ (t << 2) ^ (t << 3);
+}
+
 // splitmix64 finaliser: a bijective 64-bit mix.
 IFR_DEV uint64_t mix64(uint64_t z) {
     z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;

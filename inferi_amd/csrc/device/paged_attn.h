@@ -126,6 +126,11 @@ IFR_DEV bool pa_odd_any(uint32_t acc) { return (acc & 0xFFFFu) >= 0x7C00u || acc
 
 IFR_DEV bool pa_odd(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; } // infinite or NaN
 
+// The power of two that a query row of largest value mx is scaled by before it
+// is split: its largest value comes into [2^14, 2^15), so that the second
+// parts of values down to 2^-17 of it are normal f16 numbers.
+IFR_DEV int pa_q_exponent(float mx) { return mx > 0.0f && !pa_odd(mx) ? min(14 - ilogbf(mx), 100) : 0; }
+
 // --------------------------------------------------------- 16-row kernel --
 // One workgroup of four waves per (tile, KV head, sub-group of heads, split):
 // the tile's up to 16 (query, head) rows are one side of every product, and
@@ -216,7 +221,7 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                     }
                 }
                 mx = pa_max4(mx);
-                const int ex = mx > 0.0f && !pa_odd(mx) ? min(14 - ilogbf(mx), 100) : 0;
+                const int ex = pa_q_exponent(mx);
                 rs = ldexpf(rs, -ex);
 #pragma unroll
                 for (int c = 0; c < KC; c++)
@@ -514,6 +519,321 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
         }
         __syncthreads();
     }
+}
+
+// ------------------------------------------------------------ tile kernel --
+// Chunks: a workgroup of PAT_WAVES waves per (tile, KV head, split), 32 of the
+// tile's (query, head) rows per wave, one per lane pair (lanes l and l + 32).
+// Per key tile of 64 rows, staged in LDS (two buffers, loaded from memory one
+// tile ahead, the page numbers two ahead):
+//   S^T = K Q^T      (Q^T stays in registers; v_mfma_f32_32x32x16_f16)
+//   running softmax per row in registers: a lane holds 16 of its row's 32
+//   scores per 32-key block
+//   O^T += V^T P^T   with P^T straight from the score accumulator: the product
+//   runs over the keys in the order the accumulator holds them
+// K lies in LDS as rows, V transposed; a V^T column is the key with bits 2 and
+// 3 exchanged (a lane's eight keys then lie side by side), and the rows of dims
+// 16-31 of each 32 hold their halves of 16 keys exchanged, which spreads the
+// transposing stores over the banks.
+constexpr int PAT_WAVES = 4, PAT_ROWS = 32 * PAT_WAVES, PAT_KT = 64;
+
+template <int HSP, int T>
+__device__ void pa_tile_body(const PagedAttnArgs &a) {
+    constexpr int KC = HSP / 16, DT = HSP / 32, KP = HSP + 8, VP = PAT_KT + 8, KB = PAT_KT / 32;
+    constexpr int CPK = HSP / 8;                     // 16-byte chunks of a row
+    constexpr int R = PAT_KT * CPK / (64 * PAT_WAVES); // rows a thread stages, chunk dc of each
+    static_assert(R == 2 || R == 4, "256 threads");
+    __shared__ __attribute__((aligned(16))) _Float16 ks[2][PAT_KT][KP];
+    __shared__ __attribute__((aligned(16))) _Float16 vts[2][HSP][VP];
+    // whether V of a tile holds an infinity or NaN: tile i's flag is i % 3, set
+    // while i - 1 is worked on and cleared while i + 1 is, a barrier from either
+    __shared__ uint32_t s_odd[3];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, li = lane & 31, hl = lane >> 5;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t kvh = blockIdx.x % a.n_kv, split = blockIdx.y;
+    uint32_t r, q0, row0, nrows, kv;
+    if (!pa_find(a, blockIdx.x / a.n_kv, r, q0)) return;
+    pa_request(a, r, row0, nrows, kv);
+    const PaTile t = pa_tile(a, r, row0, nrows, kv, q0);
+    const PaKeys keys = pa_keys<PAT_KT>(a, t);
+    const uint32_t C = pa_chunk(a, keys.n), i0 = split * C, i1 = min(i0 + C, keys.n);
+    const bool one = keys.n <= C;
+    if (i0 >= i1 && !(one && split == 0)) return;
+    const uint32_t hs = a.hs, G = a.G, pm = (1u << a.lp) - 1;
+    const uint32_t rr = wave * 32 + li, qi = rr / G, head = kvh * G + rr % G;
+    const bool row_ok = qi < t.nq;
+    const int32_t qpos = row_ok ? t.p0 + (int32_t)qi : -1;
+    const size_t gq = t.row0 + (row_ok ? qi : 0);
+    const uint32_t *tab = a.table + (size_t)r * a.max_pages;
+
+    half8v qh[KC], ql[T == PA_M ? KC : 1];
+    float rs = a.scale2;
+    {
+        const char *qp = (const char *)a.q + (gq * a.ld_q + (size_t)head * hs) * (T == PA_H ? 2 : 4);
+        if constexpr (T == PA_H) {
+#pragma unroll
+            for (int c = 0; c < KC; c++) {
+                const uint32_t d = 16 * c + 8 * hl;
+                const bool ok = row_ok && d < hs;
+                uint4 x = *(const uint4 *)(qp + 2 * (ok ? d : 0));
+                if (!ok) x = make_uint4(0, 0, 0, 0);
+                qh[c] = __builtin_bit_cast(half8v, x);
+            }
+        } else {
+            float x[KC][8], mx = 0.0f;
+#pragma unroll
+            for (int c = 0; c < KC; c++) {
+                const uint32_t d = 16 * c + 8 * hl;
+                const bool ok = row_ok && d < hs;
+                const float4 u = *(const float4 *)(qp + 4 * (ok ? d : 0)), w = *(const float4 *)(qp + 4 * (ok ? d : 0) + 16);
+                const float y[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    x[c][e] = ok ? y[e] : 0.0f;
+                    mx = fmaxf(mx, fabsf(x[c][e]));
+                }
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const int ex = pa_q_exponent(mx);
+            rs = ldexpf(rs, -ex);
+#pragma unroll
+            for (int c = 0; c < KC; c++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    _Float16 hi, lo;
+                    pa_split(ldexpf(x[c][e], ex), hi, lo);
+                    qh[c][e] = hi;
+                    ql[c][e] = lo;
+                }
+        }
+    }
+
+    // this thread stages rows R gk .. R gk + R - 1 of a tile, dims 8 dc .. + 8:
+    // a load instruction reads 64 contiguous bytes of 16 rows
+    const uint32_t dc = (lane & 3u) + 4u * (wave % (CPK / 4));
+    const uint32_t gk = (lane >> 2) + 16u * (wave / (CPK / 4));
+    const uint32_t vcol = swap23(R * gk) ^ (16u * ((dc >> 1) & 1u));
+    const uint32_t d_ld = min(8 * dc, hs - 8);
+    const uint32_t lane_off = d_ld + (R * gk % 16) * (uint32_t)a.row_stride;
+    const uint32_t my16 = R * gk / 16; // which 16 rows of the tile
+    auto tile_of = [&](uint32_t i) { return i < keys.ns ? i : keys.lo + i - keys.ns; };
+    // pages of a tile's four blocks of 16 rows (uniform), and this thread's
+    auto pages_of = [&](uint32_t kt) {
+        auto one_of = [&](uint32_t z) { return tab[min((kt * 4 + z) >> (a.lp - 4), a.max_pages - 1)]; };
+        return make_uint4(one_of(0), one_of(1), one_of(2), one_of(3));
+    };
+    auto mine = [&](const uint4 &p) { return my16 == 0 ? p.x : my16 == 1 ? p.y : my16 == 2 ? p.z : p.w; };
+    uint4 kraw[R], vraw[R];
+    auto gload = [&](uint32_t kt, const uint4 &pages) {
+        const uint32_t page = mine(pages);
+        const size_t off = (size_t)((int64_t)(page < a.n_pages ? page : 0u) * a.page_stride + (int64_t)kvh * a.head_stride) +
+                           (size_t)(((kt * PAT_KT + 16 * my16) & pm) * (uint64_t)a.row_stride) + lane_off;
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            kraw[i] = *(const uint4 *)((const uint16_t *)a.key + off + (size_t)i * a.row_stride);
+            vraw[i] = *(const uint4 *)((const uint16_t *)a.value + off + (size_t)i * a.row_stride);
+        }
+    };
+    // a tile that some row does not see all of (uniform)
+    auto edge_of = [&](uint32_t kt) {
+        return (int32_t)(kt * PAT_KT + PAT_KT - 1) > t.p0 || (a.window && (int64_t)kt * PAT_KT <= (int64_t)t.plast - a.window);
+    };
+    auto gone_of = [&](const uint4 &p) { // bit z: block z's page is none
+        return (p.x >= a.n_pages ? 1u : 0u) | (p.y >= a.n_pages ? 2u : 0u) | (p.z >= a.n_pages ? 4u : 0u) |
+               (p.w >= a.n_pages ? 8u : 0u);
+    };
+    auto half_of = [&](const uint4 &q, int e) -> uint32_t {
+        const uint32_t w = e < 2 ? q.x : e < 4 ? q.y : e < 6 ? q.z : q.w;
+        return (e & 1) ? (w >> 16) : (w & 0xFFFFu);
+    };
+    auto lstore = [&](uint32_t b, uint32_t flag, uint32_t kt, const uint4 &pages) {
+        if (gone_of(pages) || edge_of(kt)) {
+            const uint32_t page = mine(pages);
+            // rows that no query of the tile sees have no part in the sums, whatever they hold
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                const int32_t key = (int32_t)(kt * PAT_KT + R * gk + i);
+                const bool any = page < a.n_pages && key <= t.plast &&
+                                 (!a.window || key > t.p0 - (int32_t)a.window || key < (int32_t)a.sinks);
+                if (!any) vraw[i] = make_uint4(0, 0, 0, 0);
+            }
+        }
+        {
+            uint32_t acc = 0;
+#pragma unroll
+            for (int i = 0; i < R; i++)
+                acc = pa_odd_acc(pa_odd_acc(pa_odd_acc(pa_odd_acc(acc, vraw[i].x), vraw[i].y), vraw[i].z), vraw[i].w);
+            if (pa_odd_any(acc)) s_odd[flag] = 1;
+        }
+#pragma unroll
+        for (int i = 0; i < R; i++) *(uint4 *)&ks[b][R * gk + i][8 * dc] = kraw[i];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            if constexpr (R == 4) {
+                uint2 v;
+                v.x = half_of(vraw[0], e) | half_of(vraw[1], e) << 16;
+                v.y = half_of(vraw[2], e) | half_of(vraw[3], e) << 16;
+                *(uint2 *)&vts[b][8 * dc + e][vcol] = v;
+            } else {
+                *(uint32_t *)&vts[b][8 * dc + e][vcol] = half_of(vraw[0], e) | half_of(vraw[1], e) << 16;
+            }
+        }
+    };
+
+    float16v o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    if (tid < 3) s_odd[tid] = 0;
+    if (i0 < i1) {
+        uint32_t kt = tile_of(i0), kn = tile_of(min(i0 + 1, i1 - 1)), flag = 0;
+        uint4 pages = pages_of(kt), pn = pages_of(kn);
+        gload(kt, pages);
+        __syncthreads(); // s_odd is cleared
+        lstore(0, 0, kt, pages);
+        __syncthreads();
+        for (uint32_t i = i0; i < i1; i++) {
+            const uint32_t b = (i - i0) & 1u, k0 = kt * PAT_KT;
+            gload(kn, pn); // (past the last: the last again, unused)
+            const uint32_t kn2 = tile_of(min(i + 2, i1 - 1));
+            const uint4 pn2 = pages_of(kn2);
+            float16v s[KB];
+#pragma unroll
+            for (int u = 0; u < KB; u++) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[u][e] = 0.0f;
+#pragma unroll
+                for (int c = 0; c < KC; c++) {
+                    const half8v av = *(const half8v *)&ks[b][32 * u + li][16 * c + 8 * hl];
+                    s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, qh[c], s[u], 0, 0, 0);
+                    if constexpr (T == PA_M) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, ql[c], s[u], 0, 0, 0);
+                }
+            }
+            const uint32_t gone = gone_of(pages);
+            const bool masked = gone || edge_of(kt);
+#pragma unroll
+            for (int u = 0; u < KB; u++) s[u] *= rs;
+            auto sees = [&](uint32_t at) { // row `at` of the tile
+                const int32_t key = (int32_t)(k0 + at);
+                return !(gone >> (at / 16) & 1u) && key <= qpos &&
+                       (!a.window || key > qpos - (int32_t)a.window || key < (int32_t)a.sinks);
+            };
+            if (masked) {
+#pragma unroll
+                for (int u = 0; u < KB; u++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        s[u][e] = sees(32 * u + 8 * (e / 4) + 4 * hl + e % 4) ? s[u][e] : -INFINITY;
+            }
+            float mt = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < KB; u++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) mt = fmaxf(mt, s[u][e]);
+            mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+            if (__ballot(mt > m + 8.0f)) {
+                const float mn = fmaxf(m, mt), al = mn == -INFINITY ? 0.0f : softmax_exp2(m - mn);
+                m = mn;
+                l *= al;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[d][e] *= al;
+            }
+            const float mr = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int u = 0; u < KB; u++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    s[u][e] = softmax_exp2(s[u][e] - mr);
+                    l += s[u][e];
+                }
+            if (s_odd[flag] && (masked || T == PA_M)) {
+                // infinities or NaN in rows of V that not all rows see (or whose weights are in two parts): their
+                // products one by one, for the rows that do; 0 in the matrix products
+                for (uint32_t at = 0; at < PAT_KT; at++) {
+                    // the weight of key `at` is with lane half (at >> 2) & 1, element 4 (at / 8 % 4) + at % 4 of block at / 32
+                    float p = 0.0f;
+#pragma unroll
+                    for (int u = 0; u < KB; u++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) p = 32 * u + 8 * (e / 4) + e % 4 == (int)(at & ~4u) ? s[u][e] : p;
+                    p = __shfl(p, (int)(li + 32 * ((at >> 2) & 1)), 64);
+                    if (!sees(at)) continue;
+                    const uint32_t pg = tab[min((k0 + at) >> a.lp, a.max_pages - 1)]; // a page: the row is seen
+                    const _Float16 *vp = (const _Float16 *)a.value + (int64_t)pg * a.page_stride +
+                                         (int64_t)((k0 + at) & pm) * a.row_stride + (int64_t)kvh * a.head_stride;
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            const uint32_t dim = 32 * d + 8 * (e / 4) + 4 * hl + e % 4;
+                            if (dim >= hs) continue;
+                            const float vv = (float)vp[dim];
+                            if (pa_odd(vv)) o[d][e] += p * vv;
+                        }
+                }
+                __syncthreads(); // (the whole workgroup is here: s_odd and masked are its own)
+                for (uint32_t z = tid; z < HSP * PAT_KT / 2; z += 64 * PAT_WAVES) {
+                    uint32_t *w = (uint32_t *)&vts[b][z / (PAT_KT / 2)][2 * (z % (PAT_KT / 2))];
+                    if ((*w & 0x7C00u) == 0x7C00u) *w &= 0xFFFF0000u;
+                    if ((*w & 0x7C000000u) == 0x7C000000u) *w &= 0xFFFFu;
+                }
+                __syncthreads();
+            }
+#pragma unroll
+            for (int u = 0; u < KB; u++)
+#pragma unroll
+                for (int cc = 0; cc < 2; cc++) {
+                    half8v ph, pl;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float p = s[u][8 * cc + e];
+                        ph[e] = (_Float16)p;
+                        if constexpr (T == PA_M) pl[e] = (_Float16)(p - (float)ph[e]);
+                    }
+                    const uint32_t kb = (32 * u + 16 * cc + 8 * hl) ^ (16u * ((li >> 4) & 1u));
+#pragma unroll
+                    for (int d = 0; d < DT; d++) {
+                        const half8v av = *(const half8v *)&vts[b][32 * d + li][kb];
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, ph, o[d], 0, 0, 0);
+                        if constexpr (T == PA_M) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, pl, o[d], 0, 0, 0);
+                    }
+                }
+            __builtin_amdgcn_sched_barrier(0);
+            const uint32_t next = flag == 2 ? 0 : flag + 1;
+            if (i + 1 < i1) lstore(b ^ 1u, next, kn, pn);
+            if (tid == 0) s_odd[next == 2 ? 0 : next + 1] = 0;
+            __syncthreads();
+            flag = next;
+            kt = kn;
+            pages = pn;
+            kn = kn2;
+            pn = pn2;
+        }
+    }
+    l += __shfl_xor(l, 32, 64);
+    if (!row_ok) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const size_t at = (gq * ((size_t)a.n_kv * G) + head) * a.n_splits + split;
+    const size_t off = gq * a.ld_out + (size_t)head * hs;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const uint32_t dim = 32 * d + 2 * e + 4 * hl;
+            if (dim >= hs) continue;
+            const float y[4] = {o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+            if (!one) *(float4 *)(a.part_o + at * hs + dim) = make_float4(y[0], y[1], y[2], y[3]);
+            else if constexpr (T == PA_H)
+                *(uint2 *)((uint16_t *)a.out + off + dim) =
+                    make_uint2((uint32_t)f32_to_f16(y[0] * inv) | (uint32_t)f32_to_f16(y[1] * inv) << 16,
+                               (uint32_t)f32_to_f16(y[2] * inv) | (uint32_t)f32_to_f16(y[3] * inv) << 16);
+            else *(float4 *)((float *)a.out + off + dim) = make_float4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+        }
+    if (!one && hl == 0) *(float2 *)(a.part_ml + at * 2) = make_float2(m, l);
 }
 
 // Joins the splits of tiles of the kernel above (KT 32) or of the tile kernel

@@ -61,6 +61,33 @@ ifr_status check_cache(ifr_ctx *c, const char *who, ifr_paged_cache &k) {
     return IFR_OK;
 }
 
+// One kernel of the attention and, where its tiles' keys go to several
+// workgroups, the kernel that joins them.  tiles: at most; key_rows: of a key
+// tile; least: key tiles that a split is worth; want: workgroups that fill the
+// chip.
+ifr_status launch_attention(ifr_ctx *c, PagedAttnArgs &a, const char *name, const char *merge, uint64_t tiles,
+                            uint32_t key_rows, uint32_t least, uint32_t want, uint32_t max_kv) {
+    const uint64_t base = tiles * a.n_sub * a.n_kv;
+    if (!base) return IFR_OK;
+    if (base >= (1u << 23)) return c->fail(IFR_EUNSUPPORTED, "paged_attention: %llu workgroups", (unsigned long long)base);
+    uint64_t keys = max_kv; // rows that a tile reads, at most
+    if (a.window) keys = std::min<uint64_t>(keys, (uint64_t)a.window + a.sinks + a.QT + 2 * key_rows);
+    const uint64_t key_tiles = (keys + key_rows - 1) / key_rows;
+    const uint64_t heads = (uint64_t)a.n_kv * a.G, row_bytes = (uint64_t)a.n_rows * heads * (a.hs + 2) * 4;
+    uint64_t splits = (want + base - 1) / base;
+    splits = std::min(splits, (key_tiles + least - 1) / least);
+    splits = std::max<uint64_t>(1, std::min(splits, PART_BYTES_MAX / row_bytes));
+    a.n_splits = (uint32_t)splits;
+    if (splits > 1) {
+        if (ifr_status st = c->ensure_scratch(row_bytes * splits)) return st;
+        a.part_o = (float *)c->scratch;
+        a.part_ml = a.part_o + (uint64_t)a.n_rows * heads * splits * a.hs;
+    }
+    ifr_status st = c->launch(name, dim3((uint32_t)base, a.n_splits), dim3(256), 0, a);
+    if (st || splits == 1) return st;
+    return c->launch(merge, dim3((uint32_t)base), dim3(256), 0, a);
+}
+
 bool bad_ld(int64_t ld, int64_t least, int64_t unit) { return ld < least || ld % unit || ld > (1ll << 40); }
 
 } // namespace
@@ -217,36 +244,41 @@ IFR_API ifr_status ifr_paged_attention(ifr_ctx *c, const ifr_paged_cache *cache,
     const uint32_t max_new = p->max_new ? std::min(p->max_new, p->n_rows) : p->n_rows;
     const uint32_t max_kv = p->max_kv ? std::min(p->max_kv, cap) : cap;
 
-    // 16 (query, head) rows a tile; a group of more heads is cut into sub-groups of 16
-    a.heads_per = std::min(a.G, 16u);
-    a.n_sub = (a.G + 15) / 16;
-    a.QT = std::max(16 / a.G, 1u);
-    a.lo_new = 1;
-    a.hi_new = 0xFFFFFFFFu;
-    a.search = max_new > a.QT;
-    const uint64_t tiles = a.search ? p->n_rows / a.QT + std::min(p->n_requests, p->n_rows) : p->n_requests;
-    const uint64_t base = tiles * a.n_sub * a.n_kv;
-    if (base >= (1u << 23)) return c->fail(IFR_EUNSUPPORTED, "paged_attention: %llu workgroups", (unsigned long long)base);
-    uint64_t keys = max_kv; // rows that a tile reads, at most
-    if (a.window) keys = std::min<uint64_t>(keys, (uint64_t)a.window + a.sinks + a.QT + 64);
-    const uint64_t key_tiles = (keys + 31) / 32;
-    uint64_t splits = (1024 + base - 1) / base;
-    splits = std::max<uint64_t>(1, std::min(splits, (key_tiles + 7) / 8));
-    const uint64_t row_bytes = (uint64_t)p->n_rows * p->n_heads * (hs + 2) * 4;
-    splits = std::max<uint64_t>(1, std::min(splits, PART_BYTES_MAX / row_bytes));
-    a.n_splits = (uint32_t)splits;
+    // Requests of up to `few` new rows run in tiles of 16 (query, head) rows, longer
+    // ones in tiles of 128 (f32 caches, whose products run at a sixteenth of the
+    // rate and need no larger tile, and groups of more than 64 heads, always in the former).
+    const bool tiles128 = k.dtype == IFR_F16 && a.G <= 64;
+    const uint32_t QT16 = std::max(16 / a.G, 1u), few = QT16;
+    const bool rows16 = !tiles128 || max_new <= few || p->n_requests > 1;
     DeviceGuard dev(c->device);
-    if (splits > 1) {
-        if (ifr_status st = c->ensure_scratch(row_bytes * splits)) return st;
-        a.part_o = (float *)c->scratch;
-        a.part_ml = a.part_o + (uint64_t)p->n_rows * p->n_heads * splits * hs;
+    if (rows16) {
+        // a group of more than 16 heads is cut into sub-groups of 16
+        a.heads_per = std::min(a.G, 16u);
+        a.n_sub = (a.G + 15) / 16;
+        a.QT = QT16;
+        a.lo_new = 1;
+        a.hi_new = tiles128 && max_new > few ? few : 0xFFFFFFFFu;
+        a.search = !tiles128 && max_new > QT16;
+        const uint64_t tiles = a.search ? p->n_rows / a.QT + std::min(p->n_requests, p->n_rows) : p->n_requests;
+        char name[64], merge[64];
+        snprintf(name, sizeof name, "paged_rows16_%s_h%u", type, hsp);
+        snprintf(merge, sizeof merge, "paged_merge32_%s_h%u", type, hsp);
+        if (ifr_status st = launch_attention(c, a, name, merge, tiles, 32, 8, 1024, max_kv)) return st;
     }
-    char name[64];
-    snprintf(name, sizeof name, "paged_rows16_%s_h%u", type, hsp);
-    ifr_status st = c->launch(name, dim3((uint32_t)base, a.n_splits), dim3(256), 0, a);
-    if (st || splits == 1) return st;
-    snprintf(name, sizeof name, "paged_merge32_%s_h%u", type, hsp);
-    return c->launch(name, dim3((uint32_t)base), dim3(256), 0, a);
+    if (tiles128 && max_new > few) {
+        a.heads_per = a.G;
+        a.n_sub = 1;
+        a.QT = 128 / a.G;
+        a.lo_new = rows16 ? few + 1 : 1;
+        a.hi_new = 0xFFFFFFFFu;
+        a.search = 1;
+        const uint64_t tiles = p->n_rows / a.QT + std::min(p->n_requests, p->n_rows / a.lo_new);
+        char name[64], merge[64];
+        snprintf(name, sizeof name, "paged_tile_%s_h%u", type, hsp);
+        snprintf(merge, sizeof merge, "paged_merge64_%s_h%u", type, hsp);
+        if (ifr_status st = launch_attention(c, a, name, merge, tiles, 64, 4, 512, max_kv)) return st;
+    }
+    return IFR_OK;
 }
 
 } // extern "C"
