@@ -355,7 +355,7 @@ IFR_API ifr_status ifr_paged_rope_store(ifr_ctx *ctx, const ifr_paged_cache *cac
  * p = kv_len[r] - n + i and sees the rows j <= p; with window > 0 only those
  * with j > p - window or j < n_sinks.
  *   out = softmax_j(scale * q . k_j) . v_j per query head; scale 0 is
- *   1 / sqrt(head_size); query head h reads KV head h / (n_heads / n_kv_heads).
+ *   1 / sqrt(head_size), others 2^-60 to 2^14; query head h reads KV head h / (n_heads / n_kv_heads).
  * Rows that see nothing (a refused request's, p < 0, no page) are 0, and so is
  * a row none of whose scores is above -infinity; rows of no request (from
  * row_start[n_requests] on) are left as they are.  What a row does not see has no part in

@@ -202,10 +202,22 @@ IFR_DEV float rope_theta_f32(float base, float head_dim, float hs) {
     return (float)pow((double)base, (double)(-head_dim / hs));
 }
 
-// x with its bits 2 and 3 exchanged
-IFR_DEV uint32_t swap23(uint32_t x) {
-    const uint32_t t = ((x >> 2) ^ (x >> 3)) & 1u;
-    return x ^ (t << 2) ^ (t << 3);
+typedef __attribute__((address_space(3))) char lds_char_t;
+
+// LDS byte address of a pointer into a __shared__ array.
+IFR_DEV uint32_t lds_addr(const void *p) { return (uint32_t)(uintptr_t)(const lds_char_t *)p; }
+
+// 16 bytes per lane from global memory straight into LDS: lane i writes
+// LDS bytes [lds + 16 i, +16) (global_load_lds_dwordx4, LDS base in M0).
+// Issued as assembly so the compiler's wait-count tracking leaves these
+// loads to the kernel's own waits; the caller waits with vmcnt before the
+// LDS is read.
+// The address is a wave-uniform base plus this lane's 32-bit byte offset.
+// M0 is reserved by the compiler (it sets M0 itself before each of its own
+// uses and ignores a clobber entry for it); the compiler-generated code of
+// these kernels does not read M0.
+IFR_DEV void lds_dma16(const void *base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds));
 }
 
 // splitmix64 finaliser: a bijective 64-bit mix.

@@ -56,6 +56,13 @@ IFR_DEV void pa_request(const PagedAttnArgs &a, uint32_t r, uint32_t &row0, uint
     n = min(max(a.row_start[r + 1], row0), a.n_rows) - row0;
     kv = min(a.kv_len[r], a.max_pages << a.lp);
 }
+// The same for a request that all lanes share (in scalar registers).
+IFR_DEV void pa_request_uniform(const PagedAttnArgs &a, uint32_t r, uint32_t &row0, uint32_t &n, uint32_t &kv) {
+    pa_request(a, r, row0, n, kv);
+    row0 = __builtin_amdgcn_readfirstlane(row0);
+    n = __builtin_amdgcn_readfirstlane(n);
+    kv = __builtin_amdgcn_readfirstlane(kv);
+}
 // Queries [q0, q0 + QT) of request r's n rows from row0.
 IFR_DEV PaTile pa_tile(const PagedAttnArgs &a, uint32_t r, uint32_t row0, uint32_t n, uint32_t kv, uint32_t q0) {
     PaTile t;
@@ -109,6 +116,13 @@ IFR_DEV float pa_sum4(float v) {
     return attn_groups_reduce<128>(v, [](float x, float y) { return x + y; });
 }
 
+// element i of an f32 or f16 array
+template <bool F32>
+IFR_DEV float pa_at(const void *p, size_t i) {
+    if constexpr (F32) return ((const float *)p)[i];
+    else return (float)((const _Float16 *)p)[i];
+}
+
 // x in two f16 parts: 22 bits of it (both parts rounded to nearest)
 IFR_DEV void pa_split(float x, _Float16 &hi, _Float16 &lo) {
     hi = (_Float16)x;
@@ -128,8 +142,9 @@ IFR_DEV bool pa_odd(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F
 
 // The power of two that a query row of largest value mx is scaled by before it
 // is split: its largest value comes into [2^14, 2^15), so that the second
-// parts of values down to 2^-17 of it are normal f16 numbers.
-IFR_DEV int pa_q_exponent(float mx) { return mx > 0.0f && !pa_odd(mx) ? min(14 - ilogbf(mx), 100) : 0; }
+// parts of values down to 2^-17 of it are normal f16 numbers.  (A row below
+// 2^-46 keeps a factor of 2^60, so that the scores' factor, its inverse, does not vanish.)
+IFR_DEV int pa_q_exponent(float mx) { return mx > 0.0f && !pa_odd(mx) ? min(14 - ilogbf(mx), 60) : 0; }
 
 // --------------------------------------------------------- 16-row kernel --
 // One workgroup of four waves per (tile, KV head, sub-group of heads, split):
@@ -172,7 +187,7 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
     const uint32_t hs = a.hs, heads = min(a.heads_per, a.G - sub * a.heads_per);
     uint32_t r = b, q0 = 0, row0, nrows, kv;
     if (a.search && !pa_find(a, b, r, q0)) return;
-    pa_request(a, r, row0, nrows, kv);
+    pa_request_uniform(a, r, row0, nrows, kv);
     if (nrows < a.lo_new || nrows > a.hi_new) return;
     const uint32_t qend = a.search ? q0 + 1 : nrows;
     const uint32_t *tab = a.table + (size_t)r * a.max_pages;
@@ -187,7 +202,9 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
         const bool one = keys.n <= C; // (a tile without keys too: split 0 writes its zeros)
         if (i0 >= i1 && !(one && split == 0)) continue;
         const bool row_ok = qi < t.nq;
-        const int32_t qpos = row_ok ? t.p0 + (int32_t)qi : -1;
+        // a row sees the keys k <= qpos with k > qlow or k < sinks
+        const int32_t qpos = row_ok ? t.p0 + (int32_t)qi : -1, sinks = (int32_t)a.sinks;
+        const int32_t qlow = a.window ? qpos - (int32_t)a.window : -1, tlow = a.window ? t.p0 - (int32_t)a.window : -1;
         const uint32_t gq = t.row0 + (row_ok ? qi : 0); // packed row
 
         // q: dims 32c + 8g .. of row n (f32 cache: 16c + 4g ..)
@@ -244,13 +261,13 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
         }
 
         float4v o[DV];
-#pragma unroll
-        for (int d = 0; d < DV; d++) o[d] = float4v{0, 0, 0, 0};
-        float m = -INFINITY, l = 0.0f;
+        float m, l;
 
         auto tile_of = [&](uint32_t i) { return i < keys.ns ? i : keys.lo + i - keys.ns; };
         // page of the 16 rows from 16 * b16
-        auto page_of = [&](uint32_t b16) { return tab[min(b16 >> (a.lp - 4), a.max_pages - 1)]; };
+        auto page_of = [&](uint32_t b16) {
+            return (uint32_t)__builtin_amdgcn_readfirstlane(tab[min(b16 >> (a.lp - 4), a.max_pages - 1)]);
+        };
         PaRegs<HSP, T> x;
         const uint32_t dk = T == PA_S ? 4 * g : 8 * g, dv = DV * n;
         auto base_of = [&](const void *p, uint32_t page, uint32_t row) {
@@ -293,6 +310,9 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
             }
         };
 
+        // The wave's tiles; false where one's V holds an infinity or NaN that the products would carry into
+        // rows that do not see it.
+        auto run = [&]() -> bool {
         uint32_t i = i0 + wave;
         if (i < i1) {
             uint32_t kt = tile_of(i), pg0 = page_of(2 * kt), pg1 = page_of(2 * kt + 1);
@@ -338,18 +358,16 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                 for (int u = 0; u < 2; u++) s[u] *= rs;
                 if (partly) {
 #pragma unroll
-                    for (int u = 0; u < 2; u++)
+                    for (int u = 0; u < 2; u++) {
+                        const bool gone = u ? bad1 : bad0;
+                        const int32_t hi = gone ? -1 : qpos, thi = gone ? -1 : t.plast;
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const int32_t key = (int32_t)(k0 + 16 * u + 4 * g + e);
-                            const bool page_ok = !(u ? bad1 : bad0);
-                            const bool see = page_ok && key <= qpos &&
-                                             (!a.window || key > qpos - (int32_t)a.window || key < (int32_t)a.sinks);
-                            s[u][e] = see ? s[u][e] : -INFINITY;
+                            s[u][e] = (key <= hi) & ((key > qlow) | (key < sinks)) ? s[u][e] : -INFINITY;
                             // a key that no row sees has no part in the sums, whatever it holds; one that
                             // some rows see and others do not must be finite to be multiplied by 0
-                            const bool any = page_ok && key <= t.plast &&
-                                             (!a.window || key > t.p0 - (int32_t)a.window || key < (int32_t)a.sinks);
+                            const bool any = (key <= thi) & ((key > tlow) | (key < sinks));
 #pragma unroll
                             for (int z = 0; z < (int)(sizeof(x.v[0]) / 4); z++) {
                                 uint32_t &w = x.v[4 * u + e][z];
@@ -357,6 +375,7 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                                 if constexpr (T == PA_S) fix |= (w & 0x7F800000u) == 0x7F800000u;
                             }
                         }
+                    }
                 }
                 if constexpr (T != PA_S) {
                     // the two parts of a weight would multiply an infinity that all rows see to NaN: every tile then
@@ -395,44 +414,7 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                         p[4 * u + e] = softmax_exp2(s[u][e] - mr);
                         l += p[4 * u + e];
                     }
-                if (__ballot(fix)) {
-                    // infinities or NaN in rows of V that not all rows of the tile see: their products are
-                    // formed one by one for the rows that do, and they are 0 in the matrix products
-                    for (int j = 0; j < 8; j++)
-                        for (uint32_t gg = 0; gg < 4; gg++) {
-                            const uint32_t kr = k0 + 16 * (j >> 2) + 4 * gg + (j & 3);
-                            float pj = 0.0f;
-#pragma unroll
-                            for (int z = 0; z < 8; z++) pj = z == j ? p[z] : pj;
-                            pj = __shfl(pj, (int)(n + 16 * gg), 64);
-                            const int32_t key = (int32_t)kr;
-                            const bool see = !((j >> 2) ? bad1 : bad0) && key <= qpos &&
-                                             (!a.window || key > qpos - (int32_t)a.window || key < (int32_t)a.sinks);
-                            if (!see) continue;
-                            const char *vp = base_of(a.value, (j >> 2) ? pg1 : pg0, kr);
-#pragma unroll
-                            for (int d = 0; d < DV; d++)
-#pragma unroll
-                                for (int e = 0; e < 4; e++) {
-                                    const uint32_t dim = DV * (4 * g + e) + d;
-                                    if (dim >= hs) continue;
-                                    const float vv = T == PA_S ? ((const float *)vp)[dim] : (float)((const _Float16 *)vp)[dim];
-                                    if (pa_odd(vv)) o[d][e] += pj * vv;
-                                }
-                        }
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-#pragma unroll
-                        for (int z = 0; z < (int)(sizeof(x.v[0]) / 4); z++) {
-                            uint32_t &w = x.v[j][z];
-                            if constexpr (T == PA_S) {
-                                if ((w & 0x7F800000u) == 0x7F800000u) w = 0;
-                            } else {
-                                if ((w & 0x7C00u) == 0x7C00u) w &= 0xFFFF0000u;
-                                if ((w & 0x7C000000u) == 0x7C000000u) w &= 0xFFFFu;
-                            }
-                        }
-                }
+                if (__ballot(fix)) return false;
                 if constexpr (T == PA_S) {
 #pragma unroll
                     for (int j = 0; j < 8; j++)
@@ -471,6 +453,43 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                 pn0 = page_of(2 * kn);
                 pn1 = page_of(2 * kn + 1);
             }
+        }
+            return true;
+        };
+        auto clear = [&]() {
+#pragma unroll
+            for (int d = 0; d < DV; d++) o[d] = float4v{0, 0, 0, 0};
+            m = -INFINITY;
+            l = 0.0f;
+        };
+        clear();
+        if (!run()) {
+            // again, key by key on the vector units, each row with the keys that it sees
+            clear();
+            for (uint32_t i = i0 + wave; i < i1; i += PAD_WAVES)
+                for (uint32_t z = 0; z < PAD_KT; z++) {
+                    const uint32_t key = tile_of(i) * PAD_KT + z, page = page_of(key / 16);
+                    if (page >= a.n_pages || (int32_t)key > t.plast) continue;
+                    const size_t koff = (size_t)((int64_t)page * a.page_stride + (int64_t)(key & pm) * a.row_stride + (int64_t)kvh * a.head_stride);
+                    float d4 = 0.0f;
+                    for (uint32_t d = 4 * DV * g; d < min(4 * DV * (g + 1), hs); d++)
+                        d4 = fmaf(pa_at<T != PA_H>(a.q, (size_t)gq * a.ld_q + (size_t)head * hs + d), pa_at<T == PA_S>(a.key, koff + d), d4);
+                    const float s1 = pa_sum4(d4) * a.scale2;
+                    if (!((int32_t)key <= qpos & ((int32_t)key > qlow | (int32_t)key < sinks))) continue;
+                    const float mn = fmaxf(m, s1), mr = mn == -INFINITY ? 0.0f : mn;
+                    const float al = m == -INFINITY ? 0.0f : softmax_exp2(m - mr), p = softmax_exp2(s1 - mr);
+                    m = mn;
+                    // (0 x inf: a sum that was infinite stays so, or was NaN)
+                    l = l * al + p;
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+#pragma unroll
+                        for (int d = 0; d < DV; d++) {
+                            const uint32_t dim = DV * (4 * g + e) + d;
+                            o[d][e] = (al == 0.0f ? 0.0f : o[d][e] * al) + p * pa_at<T == PA_S>(a.value, koff + min(dim, hs - 1));
+                        }
+                }
+            l = g == 0 ? l : 0.0f; // summed over the row's lanes below
         }
 
         // the waves' states through LDS
@@ -522,38 +541,41 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
 }
 
 // ------------------------------------------------------------ tile kernel --
-// Chunks: a workgroup of PAT_WAVES waves per (tile, KV head, split), 32 of the
+// Chunks: a workgroup of four waves per (tile, KV head, split), 32 of the
 // tile's (query, head) rows per wave, one per lane pair (lanes l and l + 32).
-// Per key tile of 64 rows, staged in LDS (two buffers, loaded from memory one
-// tile ahead, the page numbers two ahead):
+// Per key tile of 64 rows, staged in LDS (two buffers of K and of V):
 //   S^T = K Q^T      (Q^T stays in registers; v_mfma_f32_32x32x16_f16)
 //   running softmax per row in registers: a lane holds 16 of its row's 32
 //   scores per 32-key block
 //   O^T += V^T P^T   with P^T straight from the score accumulator: the product
 //   runs over the keys in the order the accumulator holds them
-// K lies in LDS as rows, V transposed; a V^T column is the key with bits 2 and
-// 3 exchanged (a lane's eight keys then lie side by side), and the rows of dims
-// 16-31 of each 32 hold their halves of 16 keys exchanged, which spreads the
-// transposing stores over the banks.
+// With AHEAD = 1 the scores of the next tile are formed between a tile's maximum
+// and its weights (K is staged a tile further ahead than V), so that matrix
+// products that nothing waits for run beside the exponentials.
+// K and V go from the cache straight into LDS (no registers in between), as
+// rows of the tile whose 16-byte chunks are exchanged by an exclusive or with
+// the row, so that the operand reads fall on distinct banks; V^T's operands
+// are read with the transposing LDS load (lane i of 16 gets column i of four
+// rows of 16).  Wave w brings the tile's rows 16w .. 16w + 15, which lie on
+// one page.  Tiles that some row does not see all of (edges) take one more
+// pass over V in LDS, which clears the rows that none sees.
 constexpr int PAT_WAVES = 4, PAT_ROWS = 32 * PAT_WAVES, PAT_KT = 64;
 
-template <int HSP, int T>
+template <int HSP, int T, int AHEAD>
 __device__ void pa_tile_body(const PagedAttnArgs &a) {
-    constexpr int KC = HSP / 16, DT = HSP / 32, KP = HSP + 8, VP = PAT_KT + 8, KB = PAT_KT / 32;
-    constexpr int CPK = HSP / 8;                     // 16-byte chunks of a row
-    constexpr int R = PAT_KT * CPK / (64 * PAT_WAVES); // rows a thread stages, chunk dc of each
-    static_assert(R == 2 || R == 4, "256 threads");
-    __shared__ __attribute__((aligned(16))) _Float16 ks[2][PAT_KT][KP];
-    __shared__ __attribute__((aligned(16))) _Float16 vts[2][HSP][VP];
-    // whether V of a tile holds an infinity or NaN: tile i's flag is i % 3, set
-    // while i - 1 is worked on and cleared while i + 1 is, a barrier from either
-    __shared__ uint32_t s_odd[3];
+    constexpr int KC = HSP / 16, DT = HSP / 32, KB = PAT_KT / 32;
+    constexpr uint32_t RB = 2 * HSP, TB = PAT_KT * RB, CPR = HSP / 8; // bytes of a row and a tile; 16-byte chunks of a row
+    constexpr uint32_t LPI = 1024 / RB;                                 // rows one load instruction brings
+    __shared__ __attribute__((aligned(1024))) char ks[2 * TB], vs[2 * TB];
+    // 16-row blocks of a tile that are on no page, a bit each: tile i's word is
+    // i % 3, set while i - 1 is worked on, cleared while i + 1 is, a barrier from either
+    __shared__ uint32_t s_flags[3];
     const uint32_t tid = threadIdx.x, lane = tid & 63, li = lane & 31, hl = lane >> 5;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t kvh = blockIdx.x % a.n_kv, split = blockIdx.y;
     uint32_t r, q0, row0, nrows, kv;
     if (!pa_find(a, blockIdx.x / a.n_kv, r, q0)) return;
-    pa_request(a, r, row0, nrows, kv);
+    pa_request_uniform(a, r, row0, nrows, kv);
     const PaTile t = pa_tile(a, r, row0, nrows, kv, q0);
     const PaKeys keys = pa_keys<PAT_KT>(a, t);
     const uint32_t C = pa_chunk(a, keys.n), i0 = split * C, i1 = min(i0 + C, keys.n);
@@ -562,7 +584,9 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
     const uint32_t hs = a.hs, G = a.G, pm = (1u << a.lp) - 1;
     const uint32_t rr = wave * 32 + li, qi = rr / G, head = kvh * G + rr % G;
     const bool row_ok = qi < t.nq;
-    const int32_t qpos = row_ok ? t.p0 + (int32_t)qi : -1;
+    // a row sees the keys k <= qpos with k > qlow or k < sinks
+    const int32_t qpos = row_ok ? t.p0 + (int32_t)qi : -1, sinks = (int32_t)a.sinks;
+    const int32_t qlow = a.window ? qpos - (int32_t)a.window : -1, tlow = a.window ? t.p0 - (int32_t)a.window : -1;
     const size_t gq = t.row0 + (row_ok ? qi : 0);
     const uint32_t *tab = a.table + (size_t)r * a.max_pages;
 
@@ -608,211 +632,229 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
         }
     }
 
-    // this thread stages rows R gk .. R gk + R - 1 of a tile, dims 8 dc .. + 8:
-    // a load instruction reads 64 contiguous bytes of 16 rows
-    const uint32_t dc = (lane & 3u) + 4u * (wave % (CPK / 4));
-    const uint32_t gk = (lane >> 2) + 16u * (wave / (CPK / 4));
-    const uint32_t vcol = swap23(R * gk) ^ (16u * ((dc >> 1) & 1u));
-    const uint32_t d_ld = min(8 * dc, hs - 8);
-    const uint32_t lane_off = d_ld + (R * gk % 16) * (uint32_t)a.row_stride;
-    const uint32_t my16 = R * gk / 16; // which 16 rows of the tile
-    auto tile_of = [&](uint32_t i) { return i < keys.ns ? i : keys.lo + i - keys.ns; };
-    // pages of a tile's four blocks of 16 rows (uniform), and this thread's
-    auto pages_of = [&](uint32_t kt) {
-        auto one_of = [&](uint32_t z) { return tab[min((kt * 4 + z) >> (a.lp - 4), a.max_pages - 1)]; };
-        return make_uint4(one_of(0), one_of(1), one_of(2), one_of(3));
+    // Chunk c of row y of a tile lies at chunk c ^ kx(y) (V: vx(y)) of the row.
+    // K's operand reads take the same chunk of 16 consecutive rows, V's four
+    // chunks (64 bytes) of four rows.
+    auto kx = [](uint32_t y) { return HSP == 128 ? y & 15 : (y >> 1) & 7; };
+    auto vx = [](uint32_t y) { return HSP == 128 ? 4 * (y & 3) : 4 * ((y >> 1) & 1); };
+    auto tile_of = [&](uint32_t i) {
+        i = min(i, i1 - 1);
+        return i < keys.ns ? i : keys.lo + i - keys.ns;
     };
-    auto mine = [&](const uint4 &p) { return my16 == 0 ? p.x : my16 == 1 ? p.y : my16 == 2 ? p.z : p.w; };
-    uint4 kraw[R], vraw[R];
-    auto gload = [&](uint32_t kt, const uint4 &pages) {
-        const uint32_t page = mine(pages);
-        const size_t off = (size_t)((int64_t)(page < a.n_pages ? page : 0u) * a.page_stride + (int64_t)kvh * a.head_stride) +
-                           (size_t)(((kt * PAT_KT + 16 * my16) & pm) * (uint64_t)a.row_stride) + lane_off;
+    // the page of this wave's rows of tile kt
+    auto page_of = [&](uint32_t kt) {
+        return (uint32_t)__builtin_amdgcn_readfirstlane(tab[min((kt * 4 + wave) >> (a.lp - 4), a.max_pages - 1)]);
+    };
+    const uint32_t dma_row = lane / CPR, dma_chunk = lane % CPR;
+    // this wave's 16 rows of tile kt into buffer b
+    auto bring = [&](const void *from, char *to, uint32_t b, uint32_t kt, uint32_t page, bool k) {
+        const char *p = (const char *)from + 2 * ((int64_t)(page < a.n_pages ? page : 0u) * a.page_stride +
+                                                  (int64_t)((kt * PAT_KT + 16 * wave) & pm) * a.row_stride +
+                                                  (int64_t)kvh * a.head_stride);
+        const uint32_t lds = lds_addr(to) + b * TB + 16 * wave * RB;
 #pragma unroll
-        for (int i = 0; i < R; i++) {
-            kraw[i] = *(const uint4 *)((const uint16_t *)a.key + off + (size_t)i * a.row_stride);
-            vraw[i] = *(const uint4 *)((const uint16_t *)a.value + off + (size_t)i * a.row_stride);
+        for (uint32_t i = 0; i < 16 / LPI; i++) {
+            const uint32_t y = i * LPI + dma_row; // of the 16
+            // (chunks past the head size: the last one, which meets q's zeros or outputs that nobody stores)
+            const uint32_t c = min(dma_chunk ^ (k ? kx(y) : vx(y)), hs / 8 - 1);
+            lds_dma16(p, 2 * (y * (uint32_t)a.row_stride + 8 * c), lds + i * 1024);
         }
     };
     // a tile that some row does not see all of (uniform)
     auto edge_of = [&](uint32_t kt) {
         return (int32_t)(kt * PAT_KT + PAT_KT - 1) > t.p0 || (a.window && (int64_t)kt * PAT_KT <= (int64_t)t.plast - a.window);
     };
-    auto gone_of = [&](const uint4 &p) { // bit z: block z's page is none
-        return (p.x >= a.n_pages ? 1u : 0u) | (p.y >= a.n_pages ? 2u : 0u) | (p.z >= a.n_pages ? 4u : 0u) |
-               (p.w >= a.n_pages ? 8u : 0u);
-    };
-    auto half_of = [&](const uint4 &q, int e) -> uint32_t {
-        const uint32_t w = e < 2 ? q.x : e < 4 ? q.y : e < 6 ? q.z : q.w;
-        return (e & 1) ? (w >> 16) : (w & 0xFFFFu);
-    };
-    auto lstore = [&](uint32_t b, uint32_t flag, uint32_t kt, const uint4 &pages) {
-        if (gone_of(pages) || edge_of(kt)) {
-            const uint32_t page = mine(pages);
-            // rows that no query of the tile sees have no part in the sums, whatever they hold
+    uint32_t k_at[KC], v_at[DT]; // byte offsets of this lane's operands in a tile
 #pragma unroll
-            for (int i = 0; i < R; i++) {
-                const int32_t key = (int32_t)(kt * PAT_KT + R * gk + i);
-                const bool any = page < a.n_pages && key <= t.plast &&
-                                 (!a.window || key > t.p0 - (int32_t)a.window || key < (int32_t)a.sinks);
-                if (!any) vraw[i] = make_uint4(0, 0, 0, 0);
+    for (int c = 0; c < KC; c++) k_at[c] = li * RB + 16 * ((2 * c + hl) ^ kx(li));
+    {
+        const uint32_t y = (lane >> 2) & 3, col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+            v_at[d] = (4 * hl + y) * RB + 16 * ((4 * d + col / 8) ^ vx(4 * hl + y)) + 2 * (col % 8);
+    }
+    auto scores = [&](uint32_t b, float16v (&s)[KB]) {
+#pragma unroll
+        for (int u = 0; u < KB; u++) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[u][e] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < KC; c++) {
+                const half8v av = *(const half8v *)(ks + b * TB + 32 * u * RB + k_at[c]);
+                s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, qh[c], s[u], 0, 0, 0);
+                if constexpr (T == PA_M) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, ql[c], s[u], 0, 0, 0);
             }
         }
-        {
-            uint32_t acc = 0;
-#pragma unroll
-            for (int i = 0; i < R; i++)
-                acc = pa_odd_acc(pa_odd_acc(pa_odd_acc(pa_odd_acc(acc, vraw[i].x), vraw[i].y), vraw[i].z), vraw[i].w);
-            if (pa_odd_any(acc)) s_odd[flag] = 1;
-        }
-#pragma unroll
-        for (int i = 0; i < R; i++) *(uint4 *)&ks[b][R * gk + i][8 * dc] = kraw[i];
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            if constexpr (R == 4) {
-                uint2 v;
-                v.x = half_of(vraw[0], e) | half_of(vraw[1], e) << 16;
-                v.y = half_of(vraw[2], e) | half_of(vraw[3], e) << 16;
-                *(uint2 *)&vts[b][8 * dc + e][vcol] = v;
-            } else {
-                *(uint32_t *)&vts[b][8 * dc + e][vcol] = half_of(vraw[0], e) | half_of(vraw[1], e) << 16;
-            }
-        }
+    };
+    // V^T operand of 16 keys: block u, half cc, dims 32 d ..
+    auto v_of = [&](uint32_t b, int u, int cc, int d) {
+        typedef __fp16 fp16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) fp16x4 lds_fp16x4;
+        const char *p = vs + b * TB + (32 * u + 16 * cc) * RB + v_at[d];
+        const fp16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_fp16x4 *)(fp16x4 *)p);
+        const fp16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_fp16x4 *)(fp16x4 *)(p + 8 * RB));
+        return __builtin_bit_cast(half8v, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
     };
 
     float16v o[DT];
+    float m, l;
+    auto clear = [&]() {
 #pragma unroll
-    for (int d = 0; d < DT; d++)
+        for (int d = 0; d < DT; d++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    if (tid < 3) s_odd[tid] = 0;
-    if (i0 < i1) {
-        uint32_t kt = tile_of(i0), kn = tile_of(min(i0 + 1, i1 - 1)), flag = 0;
-        uint4 pages = pages_of(kt), pn = pages_of(kn);
-        gload(kt, pages);
-        __syncthreads(); // s_odd is cleared
-        lstore(0, 0, kt, pages);
-        __syncthreads();
-        for (uint32_t i = i0; i < i1; i++) {
-            const uint32_t b = (i - i0) & 1u, k0 = kt * PAT_KT;
-            gload(kn, pn); // (past the last: the last again, unused)
-            const uint32_t kn2 = tile_of(min(i + 2, i1 - 1));
-            const uint4 pn2 = pages_of(kn2);
-            float16v s[KB];
+            for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
+        m = -INFINITY;
+        l = 0.0f;
+    };
+    clear();
+    if (tid < 3) s_flags[tid] = 0;
+
+    uint32_t flag = 0, kt = 0, kt1 = 0, kt2 = 0, pg1 = 0, pg2 = 0; // tiles i, i + 1, i + 2 and the latter's pages
+    // Tile i (of buffer b), its scores s (AHEAD: formed already; next: room for tile i + 1's).  false, in all
+    // waves, where its V holds an infinity or NaN that the products would carry into rows that do not see it.
+    auto step = [&](uint32_t i, const uint32_t b, float16v (&s)[KB], float16v (&next)[KB]) -> bool {
+        const uint32_t k0 = kt * PAT_KT, nf = flag == 2 ? 0 : flag + 1;
+        // (past the last tile: the last again, unused)
+        bring(a.key, ks, AHEAD ? b : b ^ 1u, AHEAD ? kt2 : kt1, AHEAD ? pg2 : pg1, true);
+        bring(a.value, vs, b ^ 1u, kt1, pg1, false);
+        const uint32_t kt3 = tile_of(i + 3), pg3 = page_of(kt3);
+        const uint32_t f = __builtin_amdgcn_readfirstlane(s_flags[flag]);
+        if (pg1 >= a.n_pages && lane == 0) atomicOr(&s_flags[nf], 1u << wave);
+        if constexpr (!AHEAD) scores(b, s);
+        const bool masked = f || edge_of(kt);
+        if (masked) {
 #pragma unroll
-            for (int u = 0; u < KB; u++) {
+            for (int z = 0; z < 4; z++) { // 16 rows on one page
+                const int32_t hi = f >> z & 1u ? -1 : qpos, base = (int32_t)(k0 + 16 * z + 4 * hl);
 #pragma unroll
-                for (int e = 0; e < 16; e++) s[u][e] = 0.0f;
-#pragma unroll
-                for (int c = 0; c < KC; c++) {
-                    const half8v av = *(const half8v *)&ks[b][32 * u + li][16 * c + 8 * hl];
-                    s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, qh[c], s[u], 0, 0, 0);
-                    if constexpr (T == PA_M) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, ql[c], s[u], 0, 0, 0);
+                for (int e = 0; e < 8; e++) {
+                    const int32_t key = base + 8 * (e / 4) + e % 4;
+                    const bool see = (key <= hi) & ((key > qlow) | (key < sinks));
+                    s[z / 2][8 * (z % 2) + e] = see ? s[z / 2][8 * (z % 2) + e] : -INFINITY;
                 }
             }
-            const uint32_t gone = gone_of(pages);
-            const bool masked = gone || edge_of(kt);
+        }
+        float mt = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < KB; u++) s[u] *= rs;
-            auto sees = [&](uint32_t at) { // row `at` of the tile
+        for (int u = 0; u < KB; u++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) mt = fmaxf(mt, s[u][e]);
+        mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * rs;
+        if (__ballot(mt > m + 8.0f)) {
+            const float mn = fmaxf(m, mt), al = mn == -INFINITY ? 0.0f : softmax_exp2(m - mn);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[d][e] *= al;
+        }
+        const float mr = m == -INFINITY ? 0.0f : m;
+        bool odd_v = false;
+        if (masked || T == PA_M) { // (the same in all waves)
+            // rows of V that no query of the tile sees have no part in the sums, whatever they hold.  (The two
+            // parts of a weight would multiply an infinity that all rows see to NaN: PA_M looks at every tile.)
+            uint32_t acc = 0;
+            for (uint32_t z = tid; z < PAT_KT * CPR; z += 64 * PAT_WAVES) {
+                uint4 *w = (uint4 *)(vs + b * TB + 16 * z);
+                const uint32_t at = z / CPR;
                 const int32_t key = (int32_t)(k0 + at);
-                return !(gone >> (at / 16) & 1u) && key <= qpos &&
-                       (!a.window || key > qpos - (int32_t)a.window || key < (int32_t)a.sinks);
-            };
-            if (masked) {
-#pragma unroll
-                for (int u = 0; u < KB; u++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        s[u][e] = sees(32 * u + 8 * (e / 4) + 4 * hl + e % 4) ? s[u][e] : -INFINITY;
+                if (!masked || (!(f >> (at / 16) & 1u) & (key <= t.plast) & ((key > tlow) | (key < sinks))))
+                    acc = pa_odd_acc(pa_odd_acc(pa_odd_acc(pa_odd_acc(acc, w->x), w->y), w->z), w->w);
+                else *w = make_uint4(0, 0, 0, 0);
             }
-            float mt = -INFINITY;
+            odd_v = __syncthreads_or(pa_odd_any(acc));
+        }
+        if (odd_v) return false;
+        if constexpr (AHEAD) scores(b ^ 1u, next);
+        half8v ph[KB][2], pl[T == PA_M ? KB : 1][2];
 #pragma unroll
-            for (int u = 0; u < KB; u++)
+        for (int u = 0; u < KB; u++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) mt = fmaxf(mt, s[u][e]);
-            mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-            if (__ballot(mt > m + 8.0f)) {
-                const float mn = fmaxf(m, mt), al = mn == -INFINITY ? 0.0f : softmax_exp2(m - mn);
+            for (int e = 0; e < 16; e++) {
+                const float p = softmax_exp2(fmaf(s[u][e], rs, -mr));
+                l += p;
+                ph[u][e / 8][e % 8] = (_Float16)p;
+                if constexpr (T == PA_M) pl[u][e / 8][e % 8] = (_Float16)(p - (float)ph[u][e / 8][e % 8]);
+            }
+#pragma unroll
+        for (int u = 0; u < KB; u++)
+#pragma unroll
+            for (int cc = 0; cc < 2; cc++)
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    const half8v av = v_of(b, u, cc, d);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, ph[u][cc], o[d], 0, 0, 0);
+                    if constexpr (T == PA_M) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, pl[u][cc], o[d], 0, 0, 0);
+                }
+        if (tid == 0) s_flags[nf == 2 ? 0 : nf + 1] = 0;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the rows brought above
+        __syncthreads();
+        flag = nf;
+        kt = kt1;
+        kt1 = kt2;
+        kt2 = kt3;
+        pg1 = pg2;
+        pg2 = pg3;
+        return true;
+    };
+    auto run = [&]() -> bool {
+    if (i0 < i1) {
+        kt = tile_of(i0);
+        kt1 = tile_of(i0 + 1);
+        kt2 = tile_of(i0 + 2);
+        const uint32_t pg = page_of(kt);
+        pg1 = page_of(kt1);
+        pg2 = page_of(kt2);
+        bring(a.key, ks, 0, kt, pg, true);
+        bring(a.value, vs, 0, kt, pg, false);
+        if constexpr (AHEAD) bring(a.key, ks, 1, kt1, pg1, true);
+        __syncthreads(); // the flags are cleared
+        if (pg >= a.n_pages && lane == 0) atomicOr(&s_flags[0], 1u << wave);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        float16v sa[KB], sb[KB];
+        if constexpr (AHEAD) {
+            scores(0, sa);
+            __syncthreads(); // buffer 0 of K is written next
+        }
+        for (uint32_t i = i0; i < i1; i += 2) {
+            if (!step(i, 0, sa, sb)) return false;
+            if (i + 1 < i1)
+                if (!(AHEAD ? step(i + 1, 1, sb, sa) : step(i + 1, 1, sa, sb))) return false;
+        }
+    }
+    return true;
+    };
+    if (!run()) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // rows on their way into LDS
+        // again, key by key on the vector units, each row with the keys that it sees
+        clear();
+        for (uint32_t i = i0; i < i1; i++)
+            for (uint32_t z = 0; z < PAT_KT; z++) {
+                const uint32_t key = tile_of(i) * PAT_KT + z;
+                if ((int32_t)key > t.plast) break;
+                const uint32_t page = __builtin_amdgcn_readfirstlane(tab[key >> a.lp]);
+                if (page >= a.n_pages) continue;
+                const size_t koff = (size_t)((int64_t)page * a.page_stride + (int64_t)(key & pm) * a.row_stride + (int64_t)kvh * a.head_stride);
+                float d2 = 0.0f;
+                for (uint32_t d = hl; d < hs; d += 2)
+                    d2 = fmaf(pa_at<T == PA_M>(a.q, gq * a.ld_q + (size_t)head * hs + d), pa_at<false>(a.key, koff + d), d2);
+                const float s1 = (d2 + __shfl_xor(d2, 32, 64)) * a.scale2;
+                if (!((int32_t)key <= qpos & ((int32_t)key > qlow | (int32_t)key < sinks))) continue;
+                const float mn = fmaxf(m, s1), mr = mn == -INFINITY ? 0.0f : mn;
+                const float al = m == -INFINITY ? 0.0f : softmax_exp2(m - mr), p = softmax_exp2(s1 - mr);
                 m = mn;
-                l *= al;
+                l = l * al + p;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) o[d][e] *= al;
-            }
-            const float mr = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-            for (int u = 0; u < KB; u++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    s[u][e] = softmax_exp2(s[u][e] - mr);
-                    l += s[u][e];
-                }
-            if (s_odd[flag] && (masked || T == PA_M)) {
-                // infinities or NaN in rows of V that not all rows see (or whose weights are in two parts): their
-                // products one by one, for the rows that do; 0 in the matrix products
-                for (uint32_t at = 0; at < PAT_KT; at++) {
-                    // the weight of key `at` is with lane half (at >> 2) & 1, element 4 (at / 8 % 4) + at % 4 of block at / 32
-                    float p = 0.0f;
-#pragma unroll
-                    for (int u = 0; u < KB; u++)
-#pragma unroll
-                        for (int e = 0; e < 16; e++) p = 32 * u + 8 * (e / 4) + e % 4 == (int)(at & ~4u) ? s[u][e] : p;
-                    p = __shfl(p, (int)(li + 32 * ((at >> 2) & 1)), 64);
-                    if (!sees(at)) continue;
-                    const uint32_t pg = tab[min((k0 + at) >> a.lp, a.max_pages - 1)]; // a page: the row is seen
-                    const _Float16 *vp = (const _Float16 *)a.value + (int64_t)pg * a.page_stride +
-                                         (int64_t)((k0 + at) & pm) * a.row_stride + (int64_t)kvh * a.head_stride;
-#pragma unroll
-                    for (int d = 0; d < DT; d++)
-#pragma unroll
-                        for (int e = 0; e < 16; e++) {
-                            const uint32_t dim = 32 * d + 8 * (e / 4) + 4 * hl + e % 4;
-                            if (dim >= hs) continue;
-                            const float vv = (float)vp[dim];
-                            if (pa_odd(vv)) o[d][e] += p * vv;
-                        }
-                }
-                __syncthreads(); // (the whole workgroup is here: s_odd and masked are its own)
-                for (uint32_t z = tid; z < HSP * PAT_KT / 2; z += 64 * PAT_WAVES) {
-                    uint32_t *w = (uint32_t *)&vts[b][z / (PAT_KT / 2)][2 * (z % (PAT_KT / 2))];
-                    if ((*w & 0x7C00u) == 0x7C00u) *w &= 0xFFFF0000u;
-                    if ((*w & 0x7C000000u) == 0x7C000000u) *w &= 0xFFFFu;
-                }
-                __syncthreads();
-            }
-#pragma unroll
-            for (int u = 0; u < KB; u++)
-#pragma unroll
-                for (int cc = 0; cc < 2; cc++) {
-                    half8v ph, pl;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const float p = s[u][8 * cc + e];
-                        ph[e] = (_Float16)p;
-                        if constexpr (T == PA_M) pl[e] = (_Float16)(p - (float)ph[e]);
+                    for (int e = 0; e < 16; e++) {
+                        const uint32_t dim = 32 * d + 8 * (e / 4) + 4 * hl + e % 4;
+                        o[d][e] = (al == 0.0f ? 0.0f : o[d][e] * al) + p * pa_at<false>(a.value, koff + min(dim, hs - 1));
                     }
-                    const uint32_t kb = (32 * u + 16 * cc + 8 * hl) ^ (16u * ((li >> 4) & 1u));
-#pragma unroll
-                    for (int d = 0; d < DT; d++) {
-                        const half8v av = *(const half8v *)&vts[b][32 * d + li][kb];
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, ph, o[d], 0, 0, 0);
-                        if constexpr (T == PA_M) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, pl, o[d], 0, 0, 0);
-                    }
-                }
-            __builtin_amdgcn_sched_barrier(0);
-            const uint32_t next = flag == 2 ? 0 : flag + 1;
-            if (i + 1 < i1) lstore(b ^ 1u, next, kn, pn);
-            if (tid == 0) s_odd[next == 2 ? 0 : next + 1] = 0;
-            __syncthreads();
-            flag = next;
-            kt = kn;
-            pages = pn;
-            kn = kn2;
-            pn = pn2;
-        }
+            }
+        l = hl ? 0.0f : l; // summed over the row's lanes below
     }
     l += __shfl_xor(l, 32, 64);
     if (!row_ok) return;
@@ -852,7 +894,7 @@ __device__ void pa_merge_body(const PagedAttnArgs &a) {
     const uint32_t hs = a.hs, heads = min(a.heads_per, a.G - sub * a.heads_per);
     uint32_t r = b, q0 = 0, row0, nrows, kv;
     if (a.search && !pa_find(a, b, r, q0)) return;
-    pa_request(a, r, row0, nrows, kv);
+    pa_request_uniform(a, r, row0, nrows, kv);
     if (nrows < a.lo_new || nrows > a.hi_new) return;
     const uint32_t qend = a.search ? q0 + 1 : nrows;
     for (; q0 < qend; q0 += a.QT) {
@@ -860,7 +902,7 @@ __device__ void pa_merge_body(const PagedAttnArgs &a) {
         const uint32_t n = pa_keys<KT>(a, t).n, C = pa_chunk(a, n);
         if (n <= C) continue;
         const uint32_t S = (n + C - 1) / C;
-        for (uint32_t rr = wave; rr < t.nq * heads; rr += 4) {
+        for (uint32_t rr = 4 * blockIdx.y + wave; rr < t.nq * heads; rr += 4 * gridDim.y) {
             const size_t orow = t.row0 + rr / heads, ohead = kvh * a.G + sub * a.heads_per + rr % heads;
             const size_t at = (orow * ((size_t)a.n_kv * a.G) + ohead) * a.n_splits;
             // the splits' references one a lane, then their weights

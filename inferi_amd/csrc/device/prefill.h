@@ -226,6 +226,12 @@ constexpr int PFA_KB = PFA_KT / 32;                                      // 32-k
 // moved.
 constexpr float PFA_LAZY = 8.0f;
 
+// x with its bits 2 and 3 exchanged
+IFR_DEV uint32_t swap23(uint32_t x) {
+    const uint32_t t = ((x >> 2) ^ (x >> 3)) & 1u;
+    return x ^ (t << 2) ^ (t << 3);
+}
+
 template <int HSP, bool F16>
 __device__ void pf_attn_body(const PfArgs &a) {
     constexpr int KC = HSP / 16;          // k-chunks of the scores (head dims)

@@ -85,7 +85,8 @@ ifr_status launch_attention(ifr_ctx *c, PagedAttnArgs &a, const char *name, cons
     }
     ifr_status st = c->launch(name, dim3((uint32_t)base, a.n_splits), dim3(256), 0, a);
     if (st || splits == 1) return st;
-    return c->launch(merge, dim3((uint32_t)base), dim3(256), 0, a);
+    // four rows of a tile per workgroup, one a wave
+    return c->launch(merge, dim3((uint32_t)base, (a.QT * a.heads_per + 3) / 4), dim3(256), 0, a);
 }
 
 bool bad_ld(int64_t ld, int64_t least, int64_t unit) { return ld < least || ld % unit || ld > (1ll << 40); }
@@ -207,7 +208,8 @@ IFR_API ifr_status ifr_paged_attention(ifr_ctx *c, const ifr_paged_cache *cache,
         return c->fail(IFR_EUNSUPPORTED, "paged_attention: f16 queries over an f32 cache");
     if (p->n_rows > MAX_CONTEXT || p->n_requests > MAX_CONTEXT)
         return c->fail(IFR_EINVAL, "paged_attention: %u rows of %u requests", p->n_rows, p->n_requests);
-    if (!std::isfinite(p->scale) || p->scale < 0.0f) return c->fail(IFR_EINVAL, "paged_attention: scale (0, or positive)");
+    if (!(p->scale == 0.0f || (p->scale >= 0x1p-60f && p->scale <= 0x1p14f)))
+        return c->fail(IFR_EINVAL, "paged_attention: scale (0, or 2^-60 to 2^14)");
     const int64_t qd = (int64_t)p->n_heads * hs;
     PagedAttnArgs a{};
     a.ld_q = p->ld_q ? p->ld_q : qd;

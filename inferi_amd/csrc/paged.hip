@@ -26,16 +26,16 @@ PA_ROWS16(mixed, 128, PA_M, 2)
 PA_ROWS16(f32, 64, PA_S, 2)
 PA_ROWS16(f32, 128, PA_S, 2)
 
-#define PA_TILE(NAME, HSP, T)                                                                               \
+#define PA_TILE(NAME, HSP, T, AHEAD)                                                                           \
     extern "C" __global__ void __launch_bounds__(64 * PAT_WAVES) __attribute__((amdgpu_waves_per_eu(2, 8))) \
     paged_tile_##NAME##_h##HSP(PagedAttnArgs a) {                                                           \
-        pa_tile_body<HSP, T>(a);                                                                            \
+        pa_tile_body<HSP, T, AHEAD>(a);                                                                     \
     }                                                                                                       \
     extern "C" __global__ void __launch_bounds__(256) paged_merge64_##NAME##_h##HSP(PagedAttnArgs a) {      \
         pa_merge_body<HSP, T, PAT_KT>(a);                                                                   \
     }
 
-PA_TILE(f16, 64, PA_H)
-PA_TILE(f16, 128, PA_H)
-PA_TILE(mixed, 64, PA_M)
-PA_TILE(mixed, 128, PA_M)
+PA_TILE(f16, 64, PA_H, 1)
+PA_TILE(f16, 128, PA_H, 1)
+PA_TILE(mixed, 64, PA_M, 0)
+PA_TILE(mixed, 128, PA_M, 0)
