@@ -7,25 +7,41 @@
 
 namespace ifr {
 
-// Inclusive sum over a workgroup of up to 1024 threads; `total` is the
-// workgroup's.  part: 16 entries of LDS, free again at the return.
-IFR_DEV uint64_t block_scan(uint64_t v, uint64_t *part, uint64_t &total) {
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, nw = (int)(blockDim.x + 63) >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t u = __shfl_up(v, d, 64);
-        if (lane >= d) v += u;
+// Sums that stay at the largest value instead of passing it (lengths come
+// from the caller; sums past 2^32 - 1 only have to be seen to be too large).
+IFR_DEV uint32_t add_sat(uint32_t x, uint32_t y) { return __builtin_elementwise_add_sat(x, y); }
+
+// Inclusive saturating sum over the wave, by DPP: within rows of 16, then the
+// rows' last lanes onto the rows behind them.
+IFR_DEV uint32_t wave_scan(uint32_t v) {
+    v = add_sat(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false)); // row_shr 1
+    v = add_sat(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
+    v = add_sat(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
+    v = add_sat(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
+    v = add_sat(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false)); // lane 15 of a row to the next, rows 1 and 3
+    v = add_sat(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false)); // lane 31 to rows 2 and 3
+    return v;
+}
+// Two inclusive saturating sums over a workgroup of up to 1024 threads, and
+// its totals.  part: 32 entries of LDS, free again at the return.
+IFR_DEV void block_scan2(uint32_t &x, uint32_t &y, uint32_t *part, uint32_t &total_x, uint32_t &total_y) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = (blockDim.x + 63) >> 6;
+    x = wave_scan(x);
+    y = wave_scan(y);
+    if (lane == 63) {
+        part[2 * wave] = x;
+        part[2 * wave + 1] = y;
     }
-    if (lane == 63) part[wave] = v;
     __syncthreads();
-    uint64_t before = 0;
-    total = 0;
-    for (int w = 0; w < nw; w++) {
-        if (w < wave) before += part[w];
-        total += part[w];
-    }
+    // the waves' sums, one a lane, in every wave
+    const uint32_t px = wave_scan(lane < nw ? part[2 * lane] : 0), py = wave_scan(lane < nw ? part[2 * lane + 1] : 0);
+    total_x = __builtin_amdgcn_readlane(px, 63);
+    total_y = __builtin_amdgcn_readlane(py, 63);
+    const uint32_t w = __builtin_amdgcn_readfirstlane(wave);
+    const uint32_t bx = w ? __builtin_amdgcn_readlane(px, w - 1) : 0, by = w ? __builtin_amdgcn_readlane(py, w - 1) : 0;
+    x = add_sat(x, bx);
+    y = add_sat(y, by);
     __syncthreads();
-    return before + v;
 }
 
 // Last index i < n with a[i] <= x (a[0] <= x, a non-decreasing).
@@ -39,14 +55,31 @@ IFR_DEV uint32_t last_at_most(const uint32_t *a, uint32_t n, uint32_t x) {
     return lo;
 }
 
+// The same for N consecutive x from x0, whose steps run side by side.
+template <int N>
+IFR_DEV void last_at_most_of(const uint32_t *a, uint32_t n, uint32_t x0, uint32_t (&at)[N]) {
+#pragma unroll
+    for (int z = 0; z < N; z++) at[z] = 0;
+    for (uint32_t step = 1u << (31 - __builtin_clz(n)); step; step >>= 1) {
+        uint32_t v[N];
+#pragma unroll
+        for (int z = 0; z < N; z++) v[z] = a[min(at[z] + step, n - 1)];
+#pragma unroll
+        for (int z = 0; z < N; z++)
+            if (at[z] + step < n && v[z] <= x0 + z) at[z] += step;
+    }
+}
+
 // Position and slot of row `row`, which is request r's (rows from `start` to
-// `end`; kv rows of the cache after the step, 0: not granted).
-IFR_DEV void paged_row(const PagedPlanArgs &a, uint32_t row, uint32_t r, uint32_t start, uint32_t end, uint32_t kv) {
+// `end`; kv rows of the cache after the step, 0: not granted).  page_of(i): the
+// page with the request's rows from i << lp.
+template <class F>
+IFR_DEV void paged_row(const PagedPlanArgs &a, uint32_t row, uint32_t start, uint32_t end, uint32_t kv, F page_of) {
     uint32_t pos = PG_NO_ROW;
     uint64_t slot = ~0ull;
     if (kv && row < end) {
         pos = kv - (end - start) + (row - start);
-        const uint32_t page = a.table[(size_t)r * a.max_pages + (pos >> a.lp)];
+        const uint32_t page = page_of(pos >> a.lp);
         if (page < a.n_pages) slot = ((uint64_t)page << a.lp) + (pos & ((1u << a.lp) - 1));
     }
     a.positions[row] = pos;
@@ -57,110 +90,125 @@ IFR_DEV void paged_row(const PagedPlanArgs &a, uint32_t row, uint32_t r, uint32_
 // running sums carried between them.  (One workgroup: the free list and the
 // table may be updated in place, and every request depends on the sums of
 // those before it; a step has far fewer requests than rows.)  Bound by the
-// latency of its chain: lengths, two scans, the popped pages, the rows.
+// latency of its chain: lengths, a scan, the popped pages with the pages of the
+// rows.  The rows take their pages from where they come from (the request's
+// last page, or the free list), not from the table entries written beside them.
 __device__ inline void paged_plan_body(const PagedPlanArgs &a) {
-    __shared__ uint64_t part[16];
-    __shared__ uint32_t s_start[PG_PLAN_THREADS + 1], s_off[PG_PLAN_THREADS + 1], s_held[PG_PLAN_THREADS], s_kv[PG_PLAN_THREADS];
-    const uint32_t tid = threadIdx.x, T = blockDim.x, lane = tid & 63, pm = (1u << a.lp) - 1;
-    uint64_t top = min(*a.free_count, a.n_pages);
-    const uint64_t cap = (uint64_t)a.max_pages << a.lp;
+    __shared__ uint32_t part[32], s_fresh;
+    __shared__ uint32_t s_start[PG_PLAN_THREADS + 1], s_off[PG_PLAN_THREADS], s_held[PG_PLAN_THREADS], s_kv[PG_PLAN_THREADS];
+    const uint32_t tid = threadIdx.x, T = blockDim.x, pm = (1u << a.lp) - 1;
+    const uint32_t cap = a.max_pages << a.lp; // at most 2^30
+    uint32_t top = min(*a.free_count, a.n_pages);
 
-    // released requests' pages onto the stack: a wave per request, its valid
-    // entries kept in order (s_off[i]: how many request i of the round has)
+    // Released requests' pages onto the stack, those that are pages, in order:
+    // the entries of a round's released requests one after another, four per
+    // thread and pass.
+    bool pushed = false;
     for (uint32_t base = 0; base < a.n_requests; base += T) {
         const uint32_t r = base + tid;
         uint32_t held = 0;
         if (r < a.n_requests && a.new_len[r] == PG_RELEASE)
             held = (uint32_t)min((uint64_t)a.max_pages, ((uint64_t)a.ctx_len[r] + pm) >> a.lp);
         if (!__syncthreads_or(held != 0)) continue;
-        s_held[tid] = held;
-        s_off[tid] = 0;
+        pushed = true;
+        uint32_t upto = held, none = 0, total, no;
+        block_scan2(upto, none, part, total, no);
+        s_start[tid] = upto - held;
         __syncthreads();
-        auto each = [&](bool push) {
-            for (uint32_t i = tid >> 6; i < T; i += T >> 6) {
-                const uint32_t h = s_held[i];
-                const uint32_t *row = a.table + (size_t)(base + i) * a.max_pages;
-                uint32_t n = 0;
-                for (uint32_t e = 0; e < h; e += 64) {
-                    const uint32_t page = e + lane < h ? row[e + lane] : ~0u;
-                    const uint64_t ok = __ballot(page < a.n_pages);
-                    if (push && page < a.n_pages) {
-                        const uint64_t to = top + s_start[i] + n + __popcll(ok & ((1ull << lane) - 1));
-                        if (to < a.n_pages) a.free_pages[to] = page;
-                    }
-                    n += __popcll(ok);
+        for (uint32_t first = 0; first < total; first += 4 * T) {
+            uint32_t page[4], count = 0, zero = 0, all;
+            const uint32_t i0 = first + 4 * tid;
+            uint32_t j[4];
+            last_at_most_of(s_start, T, i0, j);
+#pragma unroll
+            for (int z = 0; z < 4; z++)
+                page[z] = i0 + z < total ? a.table[(size_t)(base + j[z]) * a.max_pages + (i0 + z - s_start[j[z]])] : ~0u;
+#pragma unroll
+            for (int z = 0; z < 4; z++) count += page[z] < a.n_pages;
+            uint32_t to = count;
+            block_scan2(to, zero, part, all, no);
+            to += top - count;
+#pragma unroll
+            for (int z = 0; z < 4; z++)
+                if (page[z] < a.n_pages) {
+                    if (to < a.n_pages) a.free_pages[to] = page[z];
+                    to++;
                 }
-                if (!push && h && lane == 0) s_off[i] = n;
-            }
-        };
-        each(false);
+            top = min(top + all, a.n_pages);
+        }
         __syncthreads();
-        uint64_t total;
-        const uint32_t cnt = s_off[tid];
-        s_start[tid] = (uint32_t)(block_scan(cnt, part, total) - cnt);
-        __syncthreads();
-        each(true);
-        __syncthreads();
-        top = min(top + total, (uint64_t)a.n_pages);
     }
-    __threadfence(); // the pushed pages, read below by other waves
-    __syncthreads();
+    if (pushed) __syncthreads(); // read below by other waves of this workgroup
 
-    uint64_t rows0 = 0, need0 = 0, taken = 0;
+    // rows0: rows of the requests before the round; need0: pages that they need; taken: pages they got
+    uint32_t rows0 = 0, need0 = 0, taken = 0;
     for (uint32_t base = 0; base < a.n_requests; base += T) {
         const uint32_t r = base + tid, nr = min(T, a.n_requests - base);
         const bool in = r < a.n_requests;
         const uint32_t ctx = in ? a.ctx_len[r] : 0, nw = in ? a.new_len[r] : 0;
         const bool gone = nw == PG_RELEASE;
-        const uint64_t n = gone ? 0 : nw;
-        uint64_t total_rows, total_need;
-        const uint64_t end = rows0 + block_scan(n, part, total_rows), start = end - n;
-        const uint64_t sum = (uint64_t)ctx + n;
-        const bool fits = in && !gone && sum <= cap && end <= a.n_rows;
+        // (one row past n_rows is as good as any more: the sums then stay exact up to there)
+        const uint32_t n = gone ? 0 : min(nw, a.n_rows + 1), sum = gone ? ctx : add_sat(ctx, nw);
         const uint32_t held = (uint32_t)(((uint64_t)ctx + pm) >> a.lp);
-        const uint64_t need = fits ? ((sum + pm) >> a.lp) - held : 0;
-        const uint64_t off = need0 + block_scan(need, part, total_need) - need;
-        const bool ok = fits && (!need || off + need <= top);
+        const bool room = in && !gone && sum <= cap;
+        const uint32_t need = room ? ((sum + pm) >> a.lp) - held : 0;
+        // Rows and pages in one scan.  (A request whose rows end past n_rows counts for no pages, but all
+        // behind it end there too, so nobody asks for the sums that it is in.)
+        uint32_t end = n, off = need, total_rows, total_need;
+        if (tid == 0) s_fresh = 0;
+        block_scan2(end, off, part, total_rows, total_need);
+        end = add_sat(end, rows0);
+        off = add_sat(off, need0); // with its own
+        const uint32_t start = min(end - n, a.n_rows); // (a saturated sum's too is past n_rows)
+        const bool ok = room && end <= a.n_rows && (!need || off <= top);
         if (in) {
-            a.row_start[r] = (uint32_t)min(start, (uint64_t)a.n_rows);
-            a.kv_len[r] = ok ? (uint32_t)sum : 0u;
-            if (a.ctx_len_out) a.ctx_len_out[r] = ok ? (uint32_t)sum : gone ? 0u : ctx;
+            a.row_start[r] = start;
+            a.kv_len[r] = ok ? sum : 0u;
+            if (a.ctx_len_out) a.ctx_len_out[r] = ok ? sum : gone ? 0u : ctx;
         }
-        // the round's new table entries, one per thread: entry i of the round
-        // is request j's, the last one whose pages begin at or before i
-        const uint64_t mine = ok ? need : 0;
-        uint64_t fresh;
-        const uint64_t upto = block_scan(mine, part, fresh);
-        s_off[tid] = (uint32_t)(upto - mine);
-        s_start[tid] = (uint32_t)min(start, (uint64_t)a.n_rows);
+        // Pages are granted up to the first request that they do not reach, so a granted request's pages begin
+        // where the sum of needs does.
+        off -= need;
+        s_off[tid] = off;
+        s_start[tid] = start;
         s_held[tid] = held;
-        s_kv[tid] = ok ? (uint32_t)sum : 0u;
-        if (tid == nr - 1) s_start[nr] = (uint32_t)min(end, (uint64_t)a.n_rows);
+        s_kv[tid] = ok ? sum : 0u;
+        if (tid == nr - 1) s_start[nr] = min(end, a.n_rows);
+        if (ok && need) atomicMax(&s_fresh, off + need);
         __syncthreads();
-        for (uint64_t i = tid; i < fresh; i += T) {
-            const uint32_t j = last_at_most(s_off, nr, (uint32_t)i);
-            a.table[(size_t)(base + j) * a.max_pages + s_held[j] + (uint32_t)(i - s_off[j])] =
-                a.free_pages[top - 1 - (taken + i)];
+        const uint32_t fresh = max(s_fresh, taken);
+        // the round's new table entries, four per thread and pass: popped page i is request j's, the last one
+        // whose pages begin at or before i (one without new pages shares its place with the next)
+        for (uint32_t i = taken + 4 * tid; i < fresh; i += 4 * T) {
+            uint32_t j[4];
+            last_at_most_of(s_off, nr, i, j);
+#pragma unroll
+            for (int z = 0; z < 4; z++)
+                if (i + z < fresh)
+                    a.table[(size_t)(base + j[z]) * a.max_pages + s_held[j[z]] + (i + z - s_off[j[z]])] =
+                        a.free_pages[top - 1 - i - z];
         }
-        taken += fresh;
-        rows0 += total_rows;
-        need0 += total_need;
         if (a.rows_here) {
-            __threadfence_block();
-            __syncthreads();
             const uint32_t first = s_start[0], last = base + nr == a.n_requests ? a.n_rows : s_start[nr];
+#pragma unroll 2
             for (uint32_t row = first + tid; row < last; row += T) {
                 const uint32_t j = last_at_most(s_start, nr, row);
-                paged_row(a, row, base + j, s_start[j], s_start[j + 1], s_kv[j]);
+                paged_row(a, row, s_start[j], s_start[j + 1], s_kv[j], [&](uint32_t i) {
+                    return i < s_held[j] ? a.table[(size_t)(base + j) * a.max_pages + i]
+                                         : a.free_pages[top - 1 - (s_off[j] + i - s_held[j])];
+                });
             }
         }
+        taken = fresh;
+        rows0 = add_sat(rows0, total_rows);
+        need0 = add_sat(need0, total_need);
         __syncthreads();
     }
     if (!a.n_requests) // no request has any of the rows
-        for (uint32_t row = tid; row < a.n_rows; row += T) paged_row(a, row, 0, 0, 0, 0);
+        for (uint32_t row = tid; row < a.n_rows; row += T) paged_row(a, row, 0, 0, 0, [](uint32_t) { return 0u; });
     if (tid == 0) {
-        a.row_start[a.n_requests] = (uint32_t)min(rows0, (uint64_t)a.n_rows);
-        *a.free_count_out = (uint32_t)(top - taken);
+        a.row_start[a.n_requests] = min(rows0, a.n_rows);
+        *a.free_count_out = top - taken;
     }
 }
 
@@ -197,10 +245,12 @@ __device__ inline void paged_rows_body(const PagedPlanArgs &a) {
     for (uint32_t row = row0 + tid; row < min(row0 + PG_ROWS_PER, a.n_rows); row += 256) {
         if (row < s_start[nr] || r0 + nr == a.n_requests) {
             const uint32_t j = last_at_most(s_start, nr, row);
-            paged_row(a, row, r0 + j, s_start[j], s_start[j + 1], s_kv[j]);
+            paged_row(a, row, s_start[j], s_start[j + 1], s_kv[j],
+                      [&](uint32_t i) { return a.table[(size_t)(r0 + j) * a.max_pages + i]; });
         } else { // more requests than the window between this row and the workgroup's first
             const uint32_t r = last_at_most(a.row_start, a.n_requests, row);
-            paged_row(a, row, r, a.row_start[r], a.row_start[r + 1], a.kv_len[r]);
+            paged_row(a, row, a.row_start[r], a.row_start[r + 1], a.kv_len[r],
+                      [&](uint32_t i) { return a.table[(size_t)r * a.max_pages + i]; });
         }
     }
 }

@@ -47,8 +47,17 @@ IFR_DEV PaKeys pa_keys(const PagedAttnArgs &a, const PaTile &t) {
     k.n = k.ns + (uint32_t)t.plast / KT + 1 - k.lo;
     return k;
 }
-// Key tiles of each split: whole multiples shared evenly.
-IFR_DEV uint32_t pa_chunk(const PagedAttnArgs &a, uint32_t n) { return max((n + a.n_splits - 1) / a.n_splits, 1u); }
+// Key tiles of each split of a tile with n: the launch's chunk, or more where
+// its splits would not reach.
+IFR_DEV uint32_t pa_chunk(const PagedAttnArgs &a, uint32_t n) { return max((n + a.n_splits - 1) / a.n_splits, a.chunk); }
+
+// Entry i of a table that no kernel writes meanwhile, at an index that all
+// lanes share: a scalar load, which the waits for the rows on their way do not
+// order (a vector load here would wait for all of them).
+IFR_DEV uint32_t pa_entry(const uint32_t *p, uint32_t i) {
+    typedef const __attribute__((address_space(4))) uint32_t const_u32;
+    return ((const_u32 *)(uintptr_t)p)[i];
+}
 
 // Rows and cache length of request r, whatever the buffers hold.
 IFR_DEV void pa_request(const PagedAttnArgs &a, uint32_t r, uint32_t &row0, uint32_t &n, uint32_t &kv) {
@@ -58,10 +67,10 @@ IFR_DEV void pa_request(const PagedAttnArgs &a, uint32_t r, uint32_t &row0, uint
 }
 // The same for a request that all lanes share (in scalar registers).
 IFR_DEV void pa_request_uniform(const PagedAttnArgs &a, uint32_t r, uint32_t &row0, uint32_t &n, uint32_t &kv) {
-    pa_request(a, r, row0, n, kv);
-    row0 = __builtin_amdgcn_readfirstlane(row0);
-    n = __builtin_amdgcn_readfirstlane(n);
-    kv = __builtin_amdgcn_readfirstlane(kv);
+    const uint32_t s0 = pa_entry(a.row_start, r), s1 = pa_entry(a.row_start, r + 1), len = pa_entry(a.kv_len, r);
+    row0 = min(s0, a.n_rows);
+    n = min(max(s1, row0), a.n_rows) - row0;
+    kv = min(len, a.max_pages << a.lp);
 }
 // Queries [q0, q0 + QT) of request r's n rows from row0.
 IFR_DEV PaTile pa_tile(const PagedAttnArgs &a, uint32_t r, uint32_t row0, uint32_t n, uint32_t kv, uint32_t q0) {
@@ -74,35 +83,76 @@ IFR_DEV PaTile pa_tile(const PagedAttnArgs &a, uint32_t r, uint32_t row0, uint32
     t.plast = t.p0 + (int32_t)t.nq - 1;
     return t;
 }
-// The `at`-th tile, counted from the last, of all requests that the launch
-// serves; false if there are fewer.  64 requests a step, one a lane.
+IFR_DEV uint32_t pa_wave_sum(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v; // inclusive; lane 63 has the sum
+}
+// The `at`-th tile of all requests; false if there are
+// fewer.  Up to 64 requests, one a lane: the tiles in the order of their last
+// positions (by 64), the farthest first, so that the workgroups with the most
+// keys start first (nine requests' chunks, in the order of the requests 567 us).
+// More: from the last request's last tile, 64 requests a step.
 IFR_DEV bool pa_find(const PagedAttnArgs &a, uint32_t at, uint32_t &r, uint32_t &q0) {
     const uint32_t lane = threadIdx.x & 63;
+    auto pick = [&](uint32_t mine, uint32_t left, uint32_t &src, uint32_t &before) { // lane of the `left`-th of the lanes' tiles
+        const uint32_t sum = pa_wave_sum(mine);
+        const uint64_t has = __ballot(sum > left);
+        if (!has) return false;
+        src = __builtin_amdgcn_readfirstlane((uint32_t)__ffsll((unsigned long long)has) - 1);
+        before = __builtin_amdgcn_readlane(sum - mine, src);
+        return true;
+    };
+    uint32_t src = 0, before = 0;
+    if (a.n_requests <= 64) {
+        uint32_t row0, n = 0, kv = 0, nt = 0;
+        if (lane < a.n_requests) {
+            pa_request(a, lane, row0, n, kv);
+            nt = (n + a.QT - 1) / a.QT;
+        }
+        // tiles of this lane's request whose last position is 64 x or more (x = 0: all)
+        auto count = [&](uint32_t x) {
+            const int32_t least = (int32_t)(64 * x);
+            if (!x) return nt;
+            if (!nt || (int32_t)kv <= least) return 0u;
+            const int32_t up = least + 1 - (int32_t)kv + (int32_t)n; // tile c - 1 ends there if c QT reaches it
+            const uint32_t c = up > (int32_t)a.QT ? ((uint32_t)up + a.QT - 1) / a.QT : 1u;
+            return c < nt ? 1 + nt - c : 1u;
+        };
+        auto total = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane(pa_wave_sum(count(x)), 63); };
+        if (total(0) <= at) return false;
+        uint32_t lo = 0, hi = (a.max_pages << a.lp) / 64 + 1; // total(lo) > at >= total(hi)
+        while (hi - lo > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (total(mid) > at) lo = mid;
+            else hi = mid;
+        }
+        const uint32_t more = count(hi), mine = count(lo) - more;
+        if (!pick(mine, at - total(hi), src, before)) return false;
+        const uint32_t e = at - total(hi) - before + __builtin_amdgcn_readlane(more, src); // from the request's last tile
+        r = src;
+        q0 = (__builtin_amdgcn_readlane(nt, src) - 1 - e) * a.QT;
+        return true;
+    }
     uint32_t left = at;
     for (uint32_t top = a.n_requests; top;) {
         // lane 0 has the last request not yet counted
-        const uint32_t i = top - 1 - lane;
         uint32_t nt = 0;
         if (lane < top) {
             uint32_t row0, n, kv;
-            pa_request(a, i, row0, n, kv);
-            if (n >= a.lo_new && n <= a.hi_new) nt = (n + a.QT - 1) / a.QT;
+            pa_request(a, top - 1 - lane, row0, n, kv);
+            nt = (n + a.QT - 1) / a.QT;
         }
-        uint32_t sum = nt;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t u = __shfl_up(sum, d, 64);
-            if (lane >= (uint32_t)d) sum += u;
-        }
-        const uint64_t has = __ballot(sum > left);
-        if (has) {
-            const int src = __ffsll((unsigned long long)has) - 1;
-            const uint32_t s = __shfl(sum, src, 64);
-            r = __builtin_amdgcn_readfirstlane(top - 1 - (uint32_t)src);
-            q0 = __builtin_amdgcn_readfirstlane((s - 1 - left) * a.QT);
+        if (pick(nt, left, src, before)) {
+            r = top - 1 - src;
+            q0 = (__builtin_amdgcn_readlane(nt, src) - 1 - (left - before)) * a.QT;
             return true;
         }
-        left -= __shfl(sum, 63, 64);
+        left -= __builtin_amdgcn_readlane(pa_wave_sum(nt), 63);
         top -= min(top, 64u);
     }
     return false;
@@ -128,15 +178,6 @@ IFR_DEV void pa_split(float x, _Float16 &hi, _Float16 &lo) {
     hi = (_Float16)x;
     lo = (_Float16)(x - (float)hi);
 }
-
-// Whether any half of the words is infinite or NaN, collected over words: the
-// largest |half| so far in each half of acc.
-typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
-IFR_DEV uint32_t pa_odd_acc(uint32_t acc, uint32_t w) {
-    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, acc),
-                                                                  __builtin_bit_cast(ushort2v, w & 0x7FFF7FFFu)));
-}
-IFR_DEV bool pa_odd_any(uint32_t acc) { return (acc & 0xFFFFu) >= 0x7C00u || acc >= 0x7C000000u; }
 
 IFR_DEV bool pa_odd(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; } // infinite or NaN
 
@@ -188,7 +229,6 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
     uint32_t r = b, q0 = 0, row0, nrows, kv;
     if (a.search && !pa_find(a, b, r, q0)) return;
     pa_request_uniform(a, r, row0, nrows, kv);
-    if (nrows < a.lo_new || nrows > a.hi_new) return;
     const uint32_t qend = a.search ? q0 + 1 : nrows;
     const uint32_t *tab = a.table + (size_t)r * a.max_pages;
     const uint32_t pm = (1u << a.lp) - 1;
@@ -204,8 +244,72 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
         const bool row_ok = qi < t.nq;
         // a row sees the keys k <= qpos with k > qlow or k < sinks
         const int32_t qpos = row_ok ? t.p0 + (int32_t)qi : -1, sinks = (int32_t)a.sinks;
-        const int32_t qlow = a.window ? qpos - (int32_t)a.window : -1, tlow = a.window ? t.p0 - (int32_t)a.window : -1;
+        const int32_t qlow = a.window ? qpos - (int32_t)a.window : -1;
         const uint32_t gq = t.row0 + (row_ok ? qi : 0); // packed row
+
+        float4v o[DV];
+        float m, l;
+
+        auto tile_of = [&](uint32_t i) { return i < keys.ns ? i : keys.lo + i - keys.ns; };
+        // page of the 16 rows from 16 * b16
+        auto page_of = [&](uint32_t b16) {
+            return pa_entry(tab, min(b16 >> (a.lp - 4), a.max_pages - 1));
+        };
+        PaRegs<HSP, T> x;
+        const uint32_t dk = T == PA_S ? 4 * g : 8 * g, dv = DV * n;
+        auto base_of = [&](const void *p, uint32_t page, uint32_t row) {
+            return (const char *)p + ((int64_t)(page < a.n_pages ? page : 0u) * a.page_stride +
+                                      (int64_t)(row & pm) * a.row_stride + (int64_t)kvh * a.head_stride) * ES;
+        };
+        auto load_k = [&](uint32_t kt, uint32_t pg0, uint32_t pg1) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const char *p = base_of(a.key, u ? pg1 : pg0, kt * PAD_KT + 16 * u);
+                const uint32_t off = n * (uint32_t)a.row_stride;
+#pragma unroll
+                for (int c = 0; c < KC; c++) {
+                    const uint32_t d = (T == PA_S ? 16 : 32) * c + dk;
+                    x.k[u][c] = *(const uint4 *)(p + (size_t)(off + (HSP == 128 && hs == 128 ? d : min(d, hs - (T == PA_S ? 4 : 8)))) * ES);
+                }
+            }
+        };
+        auto load_v = [&](uint32_t kt, uint32_t pg0, uint32_t pg1) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const char *p = base_of(a.value, u ? pg1 : pg0, kt * PAD_KT + 16 * u);
+                const uint32_t d = min(dv, hs - DV);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const char *s = p + (size_t)((4 * g + e) * (uint32_t)a.row_stride + d) * ES;
+                    uint32_t *w = x.v[4 * u + e];
+                    constexpr int W = sizeof(x.v[0]) / 4; // 2, 4 or 8 words
+                    if constexpr (W == 2) {
+                        const uint2 y = *(const uint2 *)s;
+                        w[0] = y.x; w[1] = y.y;
+                    } else {
+#pragma unroll
+                        for (int z = 0; z < W; z += 4) {
+                            const uint4 y = *(const uint4 *)(s + 4 * z);
+                            w[z] = y.x; w[z + 1] = y.y; w[z + 2] = y.z; w[z + 3] = y.w;
+                        }
+                    }
+                }
+            }
+        };
+
+        // the first tile's rows on their way before anything else is waited for
+        uint32_t kt = 0, pg0 = 0, pg1 = 0, kn = 0, pn0 = 0, pn1 = 0;
+        if (i0 + wave < i1) {
+            kt = tile_of(i0 + wave);
+            kn = tile_of(min(i0 + wave + PAD_WAVES, i1 - 1));
+            pg0 = page_of(2 * kt);
+            pg1 = page_of(2 * kt + 1);
+            pn0 = page_of(2 * kn);
+            pn1 = page_of(2 * kn + 1);
+            load_k(kt, pg0, pg1);
+            load_v(kt, pg0, pg1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
 
         // q: dims 32c + 8g .. of row n (f32 cache: 16c + 4g ..)
         half8v qh[T == PA_S ? 1 : KC], ql[T == PA_M ? KC : 1];
@@ -260,66 +364,14 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
             }
         }
 
-        float4v o[DV];
-        float m, l;
-
-        auto tile_of = [&](uint32_t i) { return i < keys.ns ? i : keys.lo + i - keys.ns; };
-        // page of the 16 rows from 16 * b16
-        auto page_of = [&](uint32_t b16) {
-            return (uint32_t)__builtin_amdgcn_readfirstlane(tab[min(b16 >> (a.lp - 4), a.max_pages - 1)]);
+        auto clear = [&]() {
+#pragma unroll
+            for (int d = 0; d < DV; d++) o[d] = float4v{0, 0, 0, 0};
+            m = -INFINITY;
+            l = 0.0f;
         };
-        PaRegs<HSP, T> x;
-        const uint32_t dk = T == PA_S ? 4 * g : 8 * g, dv = DV * n;
-        auto base_of = [&](const void *p, uint32_t page, uint32_t row) {
-            return (const char *)p + ((int64_t)(page < a.n_pages ? page : 0u) * a.page_stride +
-                                      (int64_t)(row & pm) * a.row_stride + (int64_t)kvh * a.head_stride) * ES;
-        };
-        auto load_k = [&](uint32_t kt, uint32_t pg0, uint32_t pg1) {
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const char *p = base_of(a.key, u ? pg1 : pg0, kt * PAD_KT + 16 * u);
-                const uint32_t off = n * (uint32_t)a.row_stride;
-#pragma unroll
-                for (int c = 0; c < KC; c++) {
-                    const uint32_t d = (T == PA_S ? 16 : 32) * c + dk;
-                    x.k[u][c] = *(const uint4 *)(p + (size_t)(off + (HSP == 128 && hs == 128 ? d : min(d, hs - (T == PA_S ? 4 : 8)))) * ES);
-                }
-            }
-        };
-        auto load_v = [&](uint32_t kt, uint32_t pg0, uint32_t pg1) {
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const char *p = base_of(a.value, u ? pg1 : pg0, kt * PAD_KT + 16 * u);
-                const uint32_t d = min(dv, hs - DV);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const char *s = p + (size_t)((4 * g + e) * (uint32_t)a.row_stride + d) * ES;
-                    uint32_t *w = x.v[4 * u + e];
-                    constexpr int W = sizeof(x.v[0]) / 4; // 2, 4 or 8 words
-                    if constexpr (W == 2) {
-                        const uint2 y = *(const uint2 *)s;
-                        w[0] = y.x; w[1] = y.y;
-                    } else {
-#pragma unroll
-                        for (int z = 0; z < W; z += 4) {
-                            const uint4 y = *(const uint4 *)(s + 4 * z);
-                            w[z] = y.x; w[z + 1] = y.y; w[z + 2] = y.z; w[z + 3] = y.w;
-                        }
-                    }
-                }
-            }
-        };
-
-        // The wave's tiles; false where one's V holds an infinity or NaN that the products would carry into
-        // rows that do not see it.
-        auto run = [&]() -> bool {
-        uint32_t i = i0 + wave;
-        if (i < i1) {
-            uint32_t kt = tile_of(i), pg0 = page_of(2 * kt), pg1 = page_of(2 * kt + 1);
-            load_k(kt, pg0, pg1);
-            load_v(kt, pg0, pg1);
-            uint32_t nx = min(i + PAD_WAVES, i1 - 1), kn = tile_of(nx), pn0 = page_of(2 * kn), pn1 = page_of(2 * kn + 1);
-            for (; i < i1; i += PAD_WAVES) {
+        clear();
+            for (uint32_t i = i0 + wave; i < i1; i += PAD_WAVES) {
                 const uint32_t k0 = kt * PAD_KT;
                 if (hs != HSP) { // (uniform) dims past the head size: zero, as q's are (0 x inf is not)
 #pragma unroll
@@ -350,43 +402,33 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                 const bool bad0 = pg0 >= a.n_pages, bad1 = pg1 >= a.n_pages;
                 // the next tile's K (past the last: the last again, unused)
                 load_k(kn, pn0, pn1);
-                // keys that not every row of the tile sees
-                const bool partly = (int32_t)(k0 + PAD_KT - 1) > t.p0 ||
-                                    (a.window && (int64_t)k0 <= (int64_t)t.plast - a.window) || bad0 || bad1;
-                bool fix = false;
+                // (uniform) keys past a row's position, or on no page; keys before a row's window
+                const bool past = (int32_t)(k0 + PAD_KT - 1) > t.p0 || bad0 || bad1;
+                const bool behind = a.window && (int64_t)k0 <= (int64_t)t.plast - a.window;
 #pragma unroll
                 for (int u = 0; u < 2; u++) s[u] *= rs;
-                if (partly) {
+                if (past) {
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
                         const bool gone = u ? bad1 : bad0;
-                        const int32_t hi = gone ? -1 : qpos, thi = gone ? -1 : t.plast;
+                        const int32_t first = (int32_t)(k0 + 16 * u + 4 * g);
+                        const int32_t hi = (gone ? -1 : qpos) - first, thi = (gone ? -1 : t.plast) - first;
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            const int32_t key = (int32_t)(k0 + 16 * u + 4 * g + e);
-                            s[u][e] = (key <= hi) & ((key > qlow) | (key < sinks)) ? s[u][e] : -INFINITY;
-                            // a key that no row sees has no part in the sums, whatever it holds; one that
-                            // some rows see and others do not must be finite to be multiplied by 0
-                            const bool any = (key <= thi) & ((key > tlow) | (key < sinks));
+                            s[u][e] = e <= hi ? s[u][e] : -INFINITY;
+                            // rows of V that are on no page or past the last position have no part in the sums,
+                            // whatever was left in their memory
 #pragma unroll
-                            for (int z = 0; z < (int)(sizeof(x.v[0]) / 4); z++) {
-                                uint32_t &w = x.v[4 * u + e][z];
-                                w = any ? w : 0u;
-                                if constexpr (T == PA_S) fix |= (w & 0x7F800000u) == 0x7F800000u;
-                            }
+                            for (int z = 0; z < (int)(sizeof(x.v[0]) / 4); z++) x.v[4 * u + e][z] = e <= thi ? x.v[4 * u + e][z] : 0u;
                         }
                     }
                 }
-                if constexpr (T != PA_S) {
-                    // the two parts of a weight would multiply an infinity that all rows see to NaN: every tile then
-                    if (partly || T == PA_M) {
-                        uint32_t acc = 0;
+                if (behind) {
+                    const int32_t lo = qlow - (int32_t)(k0 + 4 * g), sk = sinks - (int32_t)(k0 + 4 * g);
 #pragma unroll
-                        for (int j = 0; j < 8; j++)
+                    for (int u = 0; u < 2; u++)
 #pragma unroll
-                            for (int z = 0; z < (int)(sizeof(x.v[0]) / 4); z++) acc = pa_odd_acc(acc, x.v[j][z]);
-                        fix = pa_odd_any(acc);
-                    }
+                        for (int e = 0; e < 4; e++) s[u][e] = (16 * u + e > lo) | (16 * u + e < sk) ? s[u][e] : -INFINITY;
                 }
                 float mt = -INFINITY;
 #pragma unroll
@@ -414,7 +456,6 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                         p[4 * u + e] = softmax_exp2(s[u][e] - mr);
                         l += p[4 * u + e];
                     }
-                if (__ballot(fix)) return false;
                 if constexpr (T == PA_S) {
 #pragma unroll
                     for (int j = 0; j < 8; j++)
@@ -448,23 +489,20 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                 load_v(kt, pn0, pn1);
                 pg0 = pn0;
                 pg1 = pn1;
-                nx = min(i + 2 * PAD_WAVES, i1 - 1);
-                kn = tile_of(nx);
+                kn = tile_of(min(i + 2 * PAD_WAVES, i1 - 1));
                 pn0 = page_of(2 * kn);
                 pn1 = page_of(2 * kn + 1);
             }
-        }
-            return true;
-        };
-        auto clear = [&]() {
+        l = pa_sum4(l);
+        // A weight of 0 times an infinity or NaN in a row of V that a query does not see is NaN (and the two parts
+        // of a weight may make one of an infinity): where a sum is not finite though its weights are, the wave does
+        // its keys again, one by one on the vector units, each row with those that it sees.
+        bool odd = false;
 #pragma unroll
-            for (int d = 0; d < DV; d++) o[d] = float4v{0, 0, 0, 0};
-            m = -INFINITY;
-            l = 0.0f;
-        };
-        clear();
-        if (!run()) {
-            // again, key by key on the vector units, each row with the keys that it sees
+        for (int d = 0; d < DV; d++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) odd |= pa_odd(o[d][e]);
+        if (__ballot(odd && row_ok && !pa_odd(l))) {
             clear();
             for (uint32_t i = i0 + wave; i < i1; i += PAD_WAVES)
                 for (uint32_t z = 0; z < PAD_KT; z++) {
@@ -489,11 +527,9 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                             o[d][e] = (al == 0.0f ? 0.0f : o[d][e] * al) + p * pa_at<T == PA_S>(a.value, koff + min(dim, hs - 1));
                         }
                 }
-            l = g == 0 ? l : 0.0f; // summed over the row's lanes below
         }
 
         // the waves' states through LDS
-        l = pa_sum4(l);
 #pragma unroll
         for (int e = 0; e < 4; e++)
 #pragma unroll
@@ -557,8 +593,7 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
 // the row, so that the operand reads fall on distinct banks; V^T's operands
 // are read with the transposing LDS load (lane i of 16 gets column i of four
 // rows of 16).  Wave w brings the tile's rows 16w .. 16w + 15, which lie on
-// one page.  Tiles that some row does not see all of (edges) take one more
-// pass over V in LDS, which clears the rows that none sees.
+// one page.
 constexpr int PAT_WAVES = 4, PAT_ROWS = 32 * PAT_WAVES, PAT_KT = 64;
 
 template <int HSP, int T, int AHEAD>
@@ -586,7 +621,7 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
     const bool row_ok = qi < t.nq;
     // a row sees the keys k <= qpos with k > qlow or k < sinks
     const int32_t qpos = row_ok ? t.p0 + (int32_t)qi : -1, sinks = (int32_t)a.sinks;
-    const int32_t qlow = a.window ? qpos - (int32_t)a.window : -1, tlow = a.window ? t.p0 - (int32_t)a.window : -1;
+    const int32_t qlow = a.window ? qpos - (int32_t)a.window : -1;
     const size_t gq = t.row0 + (row_ok ? qi : 0);
     const uint32_t *tab = a.table + (size_t)r * a.max_pages;
 
@@ -643,7 +678,7 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
     };
     // the page of this wave's rows of tile kt
     auto page_of = [&](uint32_t kt) {
-        return (uint32_t)__builtin_amdgcn_readfirstlane(tab[min((kt * 4 + wave) >> (a.lp - 4), a.max_pages - 1)]);
+        return pa_entry(tab, min((kt * 4 + wave) >> (a.lp - 4), a.max_pages - 1));
     };
     const uint32_t dma_row = lane / CPR, dma_chunk = lane % CPR;
     // this wave's 16 rows of tile kt into buffer b
@@ -659,10 +694,6 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
             const uint32_t c = min(dma_chunk ^ (k ? kx(y) : vx(y)), hs / 8 - 1);
             lds_dma16(p, 2 * (y * (uint32_t)a.row_stride + 8 * c), lds + i * 1024);
         }
-    };
-    // a tile that some row does not see all of (uniform)
-    auto edge_of = [&](uint32_t kt) {
-        return (int32_t)(kt * PAT_KT + PAT_KT - 1) > t.p0 || (a.window && (int64_t)kt * PAT_KT <= (int64_t)t.plast - a.window);
     };
     uint32_t k_at[KC], v_at[DT]; // byte offsets of this lane's operands in a tile
 #pragma unroll
@@ -710,9 +741,8 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
     if (tid < 3) s_flags[tid] = 0;
 
     uint32_t flag = 0, kt = 0, kt1 = 0, kt2 = 0, pg1 = 0, pg2 = 0; // tiles i, i + 1, i + 2 and the latter's pages
-    // Tile i (of buffer b), its scores s (AHEAD: formed already; next: room for tile i + 1's).  false, in all
-    // waves, where its V holds an infinity or NaN that the products would carry into rows that do not see it.
-    auto step = [&](uint32_t i, const uint32_t b, float16v (&s)[KB], float16v (&next)[KB]) -> bool {
+    // tile i (of buffer b), its scores s (AHEAD: formed already; next: room for tile i + 1's)
+    auto step = [&](uint32_t i, const uint32_t b, float16v (&s)[KB], float16v (&next)[KB]) {
         const uint32_t k0 = kt * PAT_KT, nf = flag == 2 ? 0 : flag + 1;
         // (past the last tile: the last again, unused)
         bring(a.key, ks, AHEAD ? b : b ^ 1u, AHEAD ? kt2 : kt1, AHEAD ? pg2 : pg1, true);
@@ -721,18 +751,37 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
         const uint32_t f = __builtin_amdgcn_readfirstlane(s_flags[flag]);
         if (pg1 >= a.n_pages && lane == 0) atomicOr(&s_flags[nf], 1u << wave);
         if constexpr (!AHEAD) scores(b, s);
-        const bool masked = f || edge_of(kt);
-        if (masked) {
+        // (uniform) keys past a row's position, or on no page; keys before a row's window
+        const bool past = f || (int32_t)(k0 + PAT_KT - 1) > t.p0;
+        const bool behind = a.window && (int64_t)k0 <= (int64_t)t.plast - a.window;
+        if (past) {
 #pragma unroll
             for (int z = 0; z < 4; z++) { // 16 rows on one page
-                const int32_t hi = f >> z & 1u ? -1 : qpos, base = (int32_t)(k0 + 16 * z + 4 * hl);
+                const int32_t hi = (f >> z & 1u ? -1 : qpos) - (int32_t)(k0 + 16 * z + 4 * hl);
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int32_t key = base + 8 * (e / 4) + e % 4;
-                    const bool see = (key <= hi) & ((key > qlow) | (key < sinks));
-                    s[z / 2][8 * (z % 2) + e] = see ? s[z / 2][8 * (z % 2) + e] : -INFINITY;
-                }
+                for (int e = 0; e < 8; e++)
+                    s[z / 2][8 * (z % 2) + e] = 8 * (e / 4) + e % 4 <= hi ? s[z / 2][8 * (z % 2) + e] : -INFINITY;
             }
+        }
+        if (behind) {
+            const int32_t lo = qlow - (int32_t)(k0 + 4 * hl), sk = sinks - (int32_t)(k0 + 4 * hl);
+#pragma unroll
+            for (int u = 0; u < KB; u++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int32_t at = 32 * u + 8 * (e / 4) + e % 4;
+                    s[u][e] = (at > lo) | (at < sk) ? s[u][e] : -INFINITY;
+                }
+        }
+        if (f || (int32_t)(k0 + PAT_KT - 1) > t.plast) {
+            // rows of V that are on no page or past the tile's last position have no part in the sums, whatever
+            // was left in their memory (the same in all waves)
+            for (uint32_t z = tid; z < PAT_KT * CPR; z += 64 * PAT_WAVES) {
+                const uint32_t at = z / CPR;
+                if ((f >> (at / 16) & 1u) || (int32_t)(k0 + at) > t.plast)
+                    *(uint4 *)(vs + b * TB + 16 * z) = make_uint4(0, 0, 0, 0);
+            }
+            __syncthreads();
         }
         float mt = -INFINITY;
 #pragma unroll
@@ -750,22 +799,6 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
                 for (int e = 0; e < 16; e++) o[d][e] *= al;
         }
         const float mr = m == -INFINITY ? 0.0f : m;
-        bool odd_v = false;
-        if (masked || T == PA_M) { // (the same in all waves)
-            // rows of V that no query of the tile sees have no part in the sums, whatever they hold.  (The two
-            // parts of a weight would multiply an infinity that all rows see to NaN: PA_M looks at every tile.)
-            uint32_t acc = 0;
-            for (uint32_t z = tid; z < PAT_KT * CPR; z += 64 * PAT_WAVES) {
-                uint4 *w = (uint4 *)(vs + b * TB + 16 * z);
-                const uint32_t at = z / CPR;
-                const int32_t key = (int32_t)(k0 + at);
-                if (!masked || (!(f >> (at / 16) & 1u) & (key <= t.plast) & ((key > tlow) | (key < sinks))))
-                    acc = pa_odd_acc(pa_odd_acc(pa_odd_acc(pa_odd_acc(acc, w->x), w->y), w->z), w->w);
-                else *w = make_uint4(0, 0, 0, 0);
-            }
-            odd_v = __syncthreads_or(pa_odd_any(acc));
-        }
-        if (odd_v) return false;
         if constexpr (AHEAD) scores(b ^ 1u, next);
         half8v ph[KB][2], pl[T == PA_M ? KB : 1][2];
 #pragma unroll
@@ -796,9 +829,7 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
         kt2 = kt3;
         pg1 = pg2;
         pg2 = pg3;
-        return true;
     };
-    auto run = [&]() -> bool {
     if (i0 < i1) {
         kt = tile_of(i0);
         kt1 = tile_of(i0 + 1);
@@ -819,16 +850,23 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
             __syncthreads(); // buffer 0 of K is written next
         }
         for (uint32_t i = i0; i < i1; i += 2) {
-            if (!step(i, 0, sa, sb)) return false;
-            if (i + 1 < i1)
-                if (!(AHEAD ? step(i + 1, 1, sb, sa) : step(i + 1, 1, sa, sb))) return false;
+            step(i, 0, sa, sb);
+            if (i + 1 < i1) {
+                if constexpr (AHEAD) step(i + 1, 1, sb, sa);
+                else step(i + 1, 1, sa, sb);
+            }
         }
     }
-    return true;
-    };
-    if (!run()) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // rows on their way into LDS
-        // again, key by key on the vector units, each row with the keys that it sees
+    // A weight of 0 times an infinity or NaN in a row of V that a query does not see is NaN (and the two parts of a
+    // weight may make one of an infinity): where a sum is not finite though its weights are, the wave does its rows
+    // again, key by key on the vector units, each row with the keys that it sees.
+    l += __shfl_xor(l, 32, 64);
+    bool odd = false;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) odd |= pa_odd(o[d][e]);
+    if (__ballot(odd && row_ok && !pa_odd(l))) {
         clear();
         for (uint32_t i = i0; i < i1; i++)
             for (uint32_t z = 0; z < PAT_KT; z++) {
@@ -854,9 +892,7 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
                         o[d][e] = (al == 0.0f ? 0.0f : o[d][e] * al) + p * pa_at<false>(a.value, koff + min(dim, hs - 1));
                     }
             }
-        l = hl ? 0.0f : l; // summed over the row's lanes below
     }
-    l += __shfl_xor(l, 32, 64);
     if (!row_ok) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const size_t at = (gq * ((size_t)a.n_kv * G) + head) * a.n_splits + split;
@@ -895,7 +931,6 @@ __device__ void pa_merge_body(const PagedAttnArgs &a) {
     uint32_t r = b, q0 = 0, row0, nrows, kv;
     if (a.search && !pa_find(a, b, r, q0)) return;
     pa_request_uniform(a, r, row0, nrows, kv);
-    if (nrows < a.lo_new || nrows > a.hi_new) return;
     const uint32_t qend = a.search ? q0 + 1 : nrows;
     for (; q0 < qend; q0 += a.QT) {
         const PaTile t = pa_tile(a, r, row0, nrows, kv, q0);

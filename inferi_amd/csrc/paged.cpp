@@ -11,6 +11,27 @@
 
 using namespace ifr;
 
+#ifndef PA_L16
+#define PA_L16 8
+#endif
+#ifndef PA_M16
+#define PA_M16 64
+#endif
+#ifndef PA_W16
+#define PA_W16 1024
+#endif
+#ifndef PA_FEW
+#define PA_FEW 2
+#endif
+#ifndef PA_L128
+#define PA_L128 4
+#endif
+#ifndef PA_M128
+#define PA_M128 1024
+#endif
+#ifndef PA_W128
+#define PA_W128 512
+#endif
 namespace {
 
 constexpr uint32_t MAX_CONTEXT = 1u << 30;          // max_pages * page_size, as max_pos
@@ -63,10 +84,10 @@ ifr_status check_cache(ifr_ctx *c, const char *who, ifr_paged_cache &k) {
 
 // One kernel of the attention and, where its tiles' keys go to several
 // workgroups, the kernel that joins them.  tiles: at most; key_rows: of a key
-// tile; least: key tiles that a split is worth; want: workgroups that fill the
-// chip.
+// tile; least, most: key tiles of a split (more only where a tile has more than
+// `most` of them for all its splits); want: workgroups that fill the chip.
 ifr_status launch_attention(ifr_ctx *c, PagedAttnArgs &a, const char *name, const char *merge, uint64_t tiles,
-                            uint32_t key_rows, uint32_t least, uint32_t want, uint32_t max_kv) {
+                            uint32_t key_rows, uint32_t least, uint32_t most, uint32_t want, uint32_t max_kv) {
     const uint64_t base = tiles * a.n_sub * a.n_kv;
     if (!base) return IFR_OK;
     if (base >= (1u << 23)) return c->fail(IFR_EUNSUPPORTED, "paged_attention: %llu workgroups", (unsigned long long)base);
@@ -74,9 +95,10 @@ ifr_status launch_attention(ifr_ctx *c, PagedAttnArgs &a, const char *name, cons
     if (a.window) keys = std::min<uint64_t>(keys, (uint64_t)a.window + a.sinks + a.QT + 2 * key_rows);
     const uint64_t key_tiles = (keys + key_rows - 1) / key_rows;
     const uint64_t heads = (uint64_t)a.n_kv * a.G, row_bytes = (uint64_t)a.n_rows * heads * (a.hs + 2) * 4;
-    uint64_t splits = (want + base - 1) / base;
-    splits = std::min(splits, (key_tiles + least - 1) / least);
-    splits = std::max<uint64_t>(1, std::min(splits, PART_BYTES_MAX / row_bytes));
+    // chunks of the keys that make `want` workgroups if all tiles are as long as the longest may be
+    uint64_t chunk = std::max<uint64_t>(least, std::min<uint64_t>(most, key_tiles * base / want));
+    uint64_t splits = std::max<uint64_t>(1, std::min((key_tiles + chunk - 1) / chunk, PART_BYTES_MAX / row_bytes));
+    a.chunk = (uint32_t)chunk;
     a.n_splits = (uint32_t)splits;
     if (splits > 1) {
         if (ifr_status st = c->ensure_scratch(row_bytes * splits)) return st;
@@ -106,6 +128,8 @@ IFR_API ifr_status ifr_paged_plan(ifr_ctx *c, const ifr_paged_plan_args *p) {
     if (p->n_rows && (!p->positions || !p->slots)) return c->fail(IFR_EINVAL, "paged_plan: null pointer");
     if (p->n_rows > MAX_CONTEXT || p->n_requests > MAX_CONTEXT)
         return c->fail(IFR_EINVAL, "paged_plan: %u rows of %u requests", p->n_rows, p->n_requests);
+    if ((uint64_t)std::min(p->n_requests, PG_PLAN_THREADS) * p->max_pages >= (1ull << 31))
+        return c->fail(IFR_EINVAL, "paged_plan: a table of %u x %u entries", p->n_requests, p->max_pages);
     DeviceGuard dev(c->device);
     PagedPlanArgs a{};
     a.ctx_len = p->ctx_len;
@@ -246,41 +270,32 @@ IFR_API ifr_status ifr_paged_attention(ifr_ctx *c, const ifr_paged_cache *cache,
     const uint32_t max_new = p->max_new ? std::min(p->max_new, p->n_rows) : p->n_rows;
     const uint32_t max_kv = p->max_kv ? std::min(p->max_kv, cap) : cap;
 
-    // Requests of up to `few` new rows run in tiles of 16 (query, head) rows, longer
-    // ones in tiles of 128 (f32 caches, whose products run at a sixteenth of the
-    // rate and need no larger tile, and groups of more than 64 heads, always in the former).
-    const bool tiles128 = k.dtype == IFR_F16 && a.G <= 64;
-    const uint32_t QT16 = std::max(16 / a.G, 1u), few = QT16;
-    const bool rows16 = !tiles128 || max_new <= few || p->n_requests > 1;
+    // Steps of up to `few` new rows a request run in tiles of 16 (query, head) rows,
+    // longer ones, with the decodes among them, in tiles of 128 (f32 caches, whose
+    // products run at a sixteenth of the rate and need no larger tile, and groups
+    // of more than 64 heads, always in the former).
+    const uint32_t QT16 = std::max(16 / a.G, 1u), few = PA_FEW * QT16;
     DeviceGuard dev(c->device);
-    if (rows16) {
+    char name[64], merge[64];
+    if (k.dtype == IFR_F32 || a.G > 64 || max_new <= few) {
         // a group of more than 16 heads is cut into sub-groups of 16
         a.heads_per = std::min(a.G, 16u);
         a.n_sub = (a.G + 15) / 16;
         a.QT = QT16;
-        a.lo_new = 1;
-        a.hi_new = tiles128 && max_new > few ? few : 0xFFFFFFFFu;
-        a.search = !tiles128 && max_new > QT16;
+        a.search = max_new > QT16;
         const uint64_t tiles = a.search ? p->n_rows / a.QT + std::min(p->n_requests, p->n_rows) : p->n_requests;
-        char name[64], merge[64];
         snprintf(name, sizeof name, "paged_rows16_%s_h%u", type, hsp);
         snprintf(merge, sizeof merge, "paged_merge32_%s_h%u", type, hsp);
-        if (ifr_status st = launch_attention(c, a, name, merge, tiles, 32, 8, 1024, max_kv)) return st;
+        return launch_attention(c, a, name, merge, tiles, 32, PA_L16, PA_M16, PA_W16, max_kv);
     }
-    if (tiles128 && max_new > few) {
-        a.heads_per = a.G;
-        a.n_sub = 1;
-        a.QT = 128 / a.G;
-        a.lo_new = rows16 ? few + 1 : 1;
-        a.hi_new = 0xFFFFFFFFu;
-        a.search = 1;
-        const uint64_t tiles = p->n_rows / a.QT + std::min(p->n_requests, p->n_rows / a.lo_new);
-        char name[64], merge[64];
-        snprintf(name, sizeof name, "paged_tile_%s_h%u", type, hsp);
-        snprintf(merge, sizeof merge, "paged_merge64_%s_h%u", type, hsp);
-        if (ifr_status st = launch_attention(c, a, name, merge, tiles, 64, 4, 512, max_kv)) return st;
-    }
-    return IFR_OK;
+    a.heads_per = a.G;
+    a.n_sub = 1;
+    a.QT = 128 / a.G;
+    a.search = 1;
+    const uint64_t tiles = p->n_rows / a.QT + std::min(p->n_requests, p->n_rows);
+    snprintf(name, sizeof name, "paged_tile_%s_h%u", type, hsp);
+    snprintf(merge, sizeof merge, "paged_merge64_%s_h%u", type, hsp);
+    return launch_attention(c, a, name, merge, tiles, 64, PA_L128, PA_M128, PA_W128, max_kv);
 }
 
 } // extern "C"

@@ -37,5 +37,5 @@ PA_ROWS16(f32, 128, PA_S, 2)
 
 PA_TILE(f16, 64, PA_H, 1)
 PA_TILE(f16, 128, PA_H, 1)
-PA_TILE(mixed, 64, PA_M, 0)
+PA_TILE(mixed, 64, PA_M, 1)
 PA_TILE(mixed, 128, PA_M, 0)

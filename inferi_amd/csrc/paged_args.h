@@ -40,10 +40,9 @@ struct PagedAttnArgs {
     int64_t ld_q, ld_out, page_stride, row_stride, head_stride;
     uint32_t n_pages, lp, max_pages, n_kv, hs, G, n_requests, n_rows;
     uint32_t window, sinks; // window 0: none
-    uint32_t n_splits;
+    uint32_t n_splits, chunk; // workgroups that share a tile's keys, at most; key tiles of each, at least
     uint32_t QT, heads_per, n_sub; // queries of a tile; heads of a sub-group; sub-groups of a KV head's heads
-    uint32_t lo_new, hi_new;       // serves the requests with lo_new <= rows <= hi_new
-    uint32_t search;               // a workgroup finds its tile among all requests' (else: tile = request)
+    uint32_t search; // a workgroup finds its tile among all requests' (else: tile = request)
     float scale2;                  // scale x log2(e)
 };
 
