@@ -92,6 +92,15 @@ IFR_DEV uint32_t pa_wave_sum(uint32_t v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
     return v; // inclusive; lane 63 has the sum
 }
+// The lane that has the `left`-th of the lanes' things (`mine` each), and how many the lanes before it have.
+IFR_DEV bool pa_pick(uint32_t mine, uint32_t left, uint32_t &src, uint32_t &before) {
+    const uint32_t sum = pa_wave_sum(mine);
+    const uint64_t has = __ballot(sum > left);
+    if (!has) return false;
+    src = __builtin_amdgcn_readfirstlane((uint32_t)__ffsll((unsigned long long)has) - 1);
+    before = __builtin_amdgcn_readlane(sum - mine, src);
+    return true;
+}
 // The `at`-th tile of all requests; false if there are
 // fewer.  Up to 64 requests, one a lane: the tiles in the order of their last
 // positions (by 64), the farthest first, so that the workgroups with the most
@@ -99,14 +108,6 @@ IFR_DEV uint32_t pa_wave_sum(uint32_t v) {
 // More: from the last request's last tile, 64 requests a step.
 IFR_DEV bool pa_find(const PagedAttnArgs &a, uint32_t at, uint32_t &r, uint32_t &q0) {
     const uint32_t lane = threadIdx.x & 63;
-    auto pick = [&](uint32_t mine, uint32_t left, uint32_t &src, uint32_t &before) { // lane of the `left`-th of the lanes' tiles
-        const uint32_t sum = pa_wave_sum(mine);
-        const uint64_t has = __ballot(sum > left);
-        if (!has) return false;
-        src = __builtin_amdgcn_readfirstlane((uint32_t)__ffsll((unsigned long long)has) - 1);
-        before = __builtin_amdgcn_readlane(sum - mine, src);
-        return true;
-    };
     uint32_t src = 0, before = 0;
     if (a.n_requests <= 64) {
         uint32_t row0, n = 0, kv = 0, nt = 0;
@@ -132,7 +133,7 @@ IFR_DEV bool pa_find(const PagedAttnArgs &a, uint32_t at, uint32_t &r, uint32_t 
             else hi = mid;
         }
         const uint32_t more = count(hi), mine = count(lo) - more;
-        if (!pick(mine, at - total(hi), src, before)) return false;
+        if (!pa_pick(mine, at - total(hi), src, before)) return false;
         const uint32_t e = at - total(hi) - before + __builtin_amdgcn_readlane(more, src); // from the request's last tile
         r = src;
         q0 = (__builtin_amdgcn_readlane(nt, src) - 1 - e) * a.QT;
@@ -147,7 +148,7 @@ IFR_DEV bool pa_find(const PagedAttnArgs &a, uint32_t at, uint32_t &r, uint32_t 
             pa_request(a, top - 1 - lane, row0, n, kv);
             nt = (n + a.QT - 1) / a.QT;
         }
-        if (pick(nt, left, src, before)) {
+        if (pa_pick(nt, left, src, before)) {
             r = top - 1 - src;
             q0 = (__builtin_amdgcn_readlane(nt, src) - 1 - (left - before)) * a.QT;
             return true;
@@ -156,6 +157,49 @@ IFR_DEV bool pa_find(const PagedAttnArgs &a, uint32_t at, uint32_t &r, uint32_t 
         top -= min(top, 64u);
     }
     return false;
+}
+
+// Key tiles of each split of request r's tiles, where a workgroup serves them all: by its last tile's keys.
+template <int KT>
+IFR_DEV uint32_t pa_request_chunk(const PagedAttnArgs &a, uint32_t r, uint32_t row0, uint32_t n, uint32_t kv, uint32_t &keys) {
+    keys = pa_keys<KT>(a, pa_tile(a, r, row0, n, kv, n ? (n - 1) / a.QT * a.QT : 0)).n;
+    return pa_chunk(a, keys);
+}
+// The `at`-th split of all requests, the longest first (whole chunks, then the
+// requests' last parts by length): workgroups of unequal lengths, the long ones
+// started last, had left the chip half empty at the end (64 decodes of 200 to
+// 8191 rows 139 us).  More than 64 requests: split by split.
+template <int KT>
+IFR_DEV bool pa_find_split(const PagedAttnArgs &a, uint32_t at, uint32_t &r, uint32_t &split) {
+    const uint32_t R = a.n_requests, lane = threadIdx.x & 63;
+    r = R == 1 ? 0 : at % R;
+    split = R == 1 ? at : at / R;
+    if (R == 1 || R > 64) return split < a.n_splits;
+    uint32_t full = 0, rest = 0; // whole chunks; key tiles of the last part, and one (0: there is none)
+    if (lane < R) {
+        uint32_t row0, n, kv, keys;
+        pa_request(a, lane, row0, n, kv);
+        const uint32_t C = pa_request_chunk<KT>(a, lane, row0, n, kv, keys);
+        full = n ? keys / C : 0;
+        rest = n && (keys % C || !full) ? keys % C + 1 : 0;
+    }
+    uint32_t src = 0, before = 0;
+    if (pa_pick(full, at, src, before)) {
+        r = src;
+        split = at - before;
+        return true;
+    }
+    const uint32_t k = at - (uint32_t)__builtin_amdgcn_readlane(pa_wave_sum(full), 63);
+    uint32_t rank = 0;
+    for (uint32_t j = 0; j < R; j++) {
+        const uint32_t other = __builtin_amdgcn_readlane(rest, j);
+        rank += (other > rest) | ((other == rest) & (j < lane));
+    }
+    const uint64_t is = __ballot(rest && rank == k);
+    if (!is) return false;
+    r = __builtin_amdgcn_readfirstlane((uint32_t)__ffsll((unsigned long long)is) - 1);
+    split = __builtin_amdgcn_readlane(full, r);
+    return true;
 }
 
 // max and sum over the four lanes of a row (lanes n, n + 16, n + 32, n + 48)
@@ -223,13 +267,13 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
     uint32_t b = blockIdx.x;
     const uint32_t kvh = b % a.n_kv;
     b /= a.n_kv;
-    const uint32_t sub = b % a.n_sub, split = blockIdx.y;
+    const uint32_t sub = b % a.n_sub;
     b /= a.n_sub;
     const uint32_t hs = a.hs, heads = min(a.heads_per, a.G - sub * a.heads_per);
-    uint32_t r = b, q0 = 0, row0, nrows, kv;
-    if (a.search && !pa_find(a, b, r, q0)) return;
+    uint32_t r, q0 = 0, split = blockIdx.y, row0, nrows, kv, last_keys;
+    if (a.search ? !pa_find(a, b, r, q0) : !pa_find_split<PAD_KT>(a, b, r, split)) return;
     pa_request_uniform(a, r, row0, nrows, kv);
-    const uint32_t qend = a.search ? q0 + 1 : nrows;
+    const uint32_t qend = a.search ? q0 + 1 : nrows, chunk = pa_request_chunk<PAD_KT>(a, r, row0, nrows, kv, last_keys);
     const uint32_t *tab = a.table + (size_t)r * a.max_pages;
     const uint32_t pm = (1u << a.lp) - 1;
     const uint32_t qi = n / heads, hj = sub * a.heads_per + n % heads; // this lane's row
@@ -238,7 +282,7 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
     for (; q0 < qend; q0 += a.QT) {
         const PaTile t = pa_tile(a, r, row0, nrows, kv, q0);
         const PaKeys keys = pa_keys<PAD_KT>(a, t);
-        const uint32_t C = pa_chunk(a, keys.n), i0 = split * C, i1 = min(i0 + C, keys.n);
+        const uint32_t C = a.search ? pa_chunk(a, keys.n) : chunk, i0 = split * C, i1 = min(i0 + C, keys.n);
         const bool one = keys.n <= C; // (a tile without keys too: split 0 writes its zeros)
         if (i0 >= i1 && !(one && split == 0)) continue;
         const bool row_ok = qi < t.nq;
@@ -585,9 +629,6 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
 //   scores per 32-key block
 //   O^T += V^T P^T   with P^T straight from the score accumulator: the product
 //   runs over the keys in the order the accumulator holds them
-// With AHEAD = 1 the scores of the next tile are formed between a tile's maximum
-// and its weights (K is staged a tile further ahead than V), so that matrix
-// products that nothing waits for run beside the exponentials.
 // K and V go from the cache straight into LDS (no registers in between), as
 // rows of the tile whose 16-byte chunks are exchanged by an exclusive or with
 // the row, so that the operand reads fall on distinct banks; V^T's operands
@@ -596,7 +637,7 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
 // one page.
 constexpr int PAT_WAVES = 4, PAT_ROWS = 32 * PAT_WAVES, PAT_KT = 64;
 
-template <int HSP, int T, int AHEAD>
+template <int HSP, int T>
 __device__ void pa_tile_body(const PagedAttnArgs &a) {
     constexpr int KC = HSP / 16, DT = HSP / 32, KB = PAT_KT / 32;
     constexpr uint32_t RB = 2 * HSP, TB = PAT_KT * RB, CPR = HSP / 8; // bytes of a row and a tile; 16-byte chunks of a row
@@ -740,17 +781,17 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
     clear();
     if (tid < 3) s_flags[tid] = 0;
 
-    uint32_t flag = 0, kt = 0, kt1 = 0, kt2 = 0, pg1 = 0, pg2 = 0; // tiles i, i + 1, i + 2 and the latter's pages
-    // tile i (of buffer b), its scores s (AHEAD: formed already; next: room for tile i + 1's)
-    auto step = [&](uint32_t i, const uint32_t b, float16v (&s)[KB], float16v (&next)[KB]) {
+    uint32_t flag = 0, kt = 0, kt1 = 0, pg1 = 0; // tiles i and i + 1, and the latter's page
+    auto step = [&](uint32_t i, const uint32_t b) { // tile i, in buffer b
+        float16v s[KB];
         const uint32_t k0 = kt * PAT_KT, nf = flag == 2 ? 0 : flag + 1;
         // (past the last tile: the last again, unused)
-        bring(a.key, ks, AHEAD ? b : b ^ 1u, AHEAD ? kt2 : kt1, AHEAD ? pg2 : pg1, true);
+        bring(a.key, ks, b ^ 1u, kt1, pg1, true);
         bring(a.value, vs, b ^ 1u, kt1, pg1, false);
-        const uint32_t kt3 = tile_of(i + 3), pg3 = page_of(kt3);
+        const uint32_t kt2 = tile_of(i + 2), pg2 = page_of(kt2);
         const uint32_t f = __builtin_amdgcn_readfirstlane(s_flags[flag]);
         if (pg1 >= a.n_pages && lane == 0) atomicOr(&s_flags[nf], 1u << wave);
-        if constexpr (!AHEAD) scores(b, s);
+        scores(b, s);
         // (uniform) keys past a row's position, or on no page; keys before a row's window
         const bool past = f || (int32_t)(k0 + PAT_KT - 1) > t.p0;
         const bool behind = a.window && (int64_t)k0 <= (int64_t)t.plast - a.window;
@@ -799,7 +840,6 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
                 for (int e = 0; e < 16; e++) o[d][e] *= al;
         }
         const float mr = m == -INFINITY ? 0.0f : m;
-        if constexpr (AHEAD) scores(b ^ 1u, next);
         half8v ph[KB][2], pl[T == PA_M ? KB : 1][2];
 #pragma unroll
         for (int u = 0; u < KB; u++)
@@ -826,35 +866,22 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
         flag = nf;
         kt = kt1;
         kt1 = kt2;
-        kt2 = kt3;
         pg1 = pg2;
-        pg2 = pg3;
     };
     if (i0 < i1) {
         kt = tile_of(i0);
         kt1 = tile_of(i0 + 1);
-        kt2 = tile_of(i0 + 2);
         const uint32_t pg = page_of(kt);
         pg1 = page_of(kt1);
-        pg2 = page_of(kt2);
         bring(a.key, ks, 0, kt, pg, true);
         bring(a.value, vs, 0, kt, pg, false);
-        if constexpr (AHEAD) bring(a.key, ks, 1, kt1, pg1, true);
         __syncthreads(); // the flags are cleared
         if (pg >= a.n_pages && lane == 0) atomicOr(&s_flags[0], 1u << wave);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        float16v sa[KB], sb[KB];
-        if constexpr (AHEAD) {
-            scores(0, sa);
-            __syncthreads(); // buffer 0 of K is written next
-        }
         for (uint32_t i = i0; i < i1; i += 2) {
-            step(i, 0, sa, sb);
-            if (i + 1 < i1) {
-                if constexpr (AHEAD) step(i + 1, 1, sb, sa);
-                else step(i + 1, 1, sa, sb);
-            }
+            step(i, 0);
+            if (i + 1 < i1) step(i + 1, 1);
         }
     }
     // A weight of 0 times an infinity or NaN in a row of V that a query does not see is NaN (and the two parts of a
@@ -914,13 +941,16 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
     if (!one && hl == 0) *(float2 *)(a.part_ml + at * 2) = make_float2(m, l);
 }
 
-// Joins the splits of tiles of the kernel above (KT 32) or of the tile kernel
-// (KT 64): grid as its x.  A wave takes a row of the tile at a time, a lane
-// the dims 2 lane, 2 lane + 1 (64 dims: one).  Only splits that the tile has are
+// Joins the splits of tiles of the 16-row kernel (KT 32, RPW 1) or of the tile
+// kernel (KT 64, RPW 4): grid as its x, and per y four waves of RPW rows of the
+// tile each.  A lane has the dims 2 lane, 2 lane + 1 (64 dims: one) of every
+// row, and one split's (m, l) of 64 at a time; the rows' loads go out together.
+// Bound by the latency of its chain (request, (m, l) with the first partials,
+// output) and then by the partials' bytes.  Only splits that the tile has are
 // read; a tile of one split is written already.
-template <int HSP, int T, int KT>
+template <int HSP, int T, int KT, int RPW>
 __device__ void pa_merge_body(const PagedAttnArgs &a) {
-    constexpr int E = HSP / 64;
+    constexpr int E = HSP / 64, U = RPW == 1 ? 16 : 4; // U: partials of a row on their way
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint32_t b = blockIdx.x;
     const uint32_t kvh = b % a.n_kv;
@@ -931,46 +961,89 @@ __device__ void pa_merge_body(const PagedAttnArgs &a) {
     uint32_t r = b, q0 = 0, row0, nrows, kv;
     if (a.search && !pa_find(a, b, r, q0)) return;
     pa_request_uniform(a, r, row0, nrows, kv);
-    const uint32_t qend = a.search ? q0 + 1 : nrows;
+    uint32_t last_keys;
+    const uint32_t qend = a.search ? q0 + 1 : nrows, chunk = pa_request_chunk<KT>(a, r, row0, nrows, kv, last_keys);
+    const uint32_t d = E * lane, dl = min(d, hs - E);
     for (; q0 < qend; q0 += a.QT) {
         const PaTile t = pa_tile(a, r, row0, nrows, kv, q0);
-        const uint32_t n = pa_keys<KT>(a, t).n, C = pa_chunk(a, n);
+        const uint32_t n = pa_keys<KT>(a, t).n, C = a.search ? pa_chunk(a, n) : chunk;
         if (n <= C) continue;
-        const uint32_t S = (n + C - 1) / C;
-        for (uint32_t rr = 4 * blockIdx.y + wave; rr < t.nq * heads; rr += 4 * gridDim.y) {
-            const size_t orow = t.row0 + rr / heads, ohead = kvh * a.G + sub * a.heads_per + rr % heads;
-            const size_t at = (orow * ((size_t)a.n_kv * a.G) + ohead) * a.n_splits;
-            // the splits' references one a lane, then their weights
-            float M = -INFINITY;
-            for (uint32_t s = lane; s < S; s += 64) M = fmaxf(M, a.part_ml[(at + s) * 2]);
-            M = wave_max(M);
-            const float mr = M == -INFINITY ? 0.0f : M;
-            float L = 0.0f;
-            for (uint32_t s = lane; s < S; s += 64)
-                L = fmaf(a.part_ml[(at + s) * 2 + 1], softmax_exp2(a.part_ml[(at + s) * 2] - mr), L);
-            L = wave_sum(L);
-            const uint32_t d = E * lane;
-            const bool in = d < hs;
-            float O[E] = {};
-            const float *po = a.part_o + at * hs + (in ? d : 0);
-#pragma unroll 8
-            for (uint32_t s = 0; s < S; s++) {
-                const float w = softmax_exp2(a.part_ml[(at + s) * 2] - mr);
-                if constexpr (E == 2) {
-                    const float2 y = *(const float2 *)(po + (size_t)s * hs);
-                    O[0] = fmaf(y.x, w, O[0]);
-                    O[1] = fmaf(y.y, w, O[1]);
-                } else {
-                    O[0] = fmaf(po[(size_t)s * hs], w, O[0]);
+        const uint32_t S = (n + C - 1) / C, rows = t.nq * heads;
+        for (uint32_t first = RPW * (4 * blockIdx.y + wave); first < rows; first += RPW * 4 * gridDim.y) {
+            size_t at[RPW];   // the row's first partial
+            size_t out[RPW];
+            float M[RPW], L[RPW], O[RPW][E];
+#pragma unroll
+            for (int k = 0; k < RPW; k++) {
+                const uint32_t rr = min(first + k, rows - 1); // (past the last row: it again)
+                const size_t orow = t.row0 + rr / heads, ohead = kvh * a.G + sub * a.heads_per + rr % heads;
+                at[k] = (orow * ((size_t)a.n_kv * a.G) + ohead) * a.n_splits;
+                out[k] = orow * a.ld_out + ohead * hs + d;
+                M[k] = -INFINITY;
+                L[k] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; e++) O[k][e] = 0.0f;
+            }
+            for (uint32_t s0 = 0; s0 < S; s0 += 64) {
+                const uint32_t nb = min(S - s0, 64u);
+                float2 ml[RPW];
+                float v[RPW][U][E];
+                auto load = [&](uint32_t s) { // (past the last: it again, unused)
+#pragma unroll
+                    for (int k = 0; k < RPW; k++)
+#pragma unroll
+                        for (int z = 0; z < U; z++) {
+                            const float *p = a.part_o + (at[k] + s0 + min(s + z, nb - 1)) * hs + dl;
+#pragma unroll
+                            for (int e = 0; e < E; e++) v[k][z][e] = p[e];
+                        }
+                };
+#pragma unroll
+                for (int k = 0; k < RPW; k++) {
+                    ml[k] = *(const float2 *)(a.part_ml + (at[k] + s0 + min(lane, nb - 1)) * 2);
+                    if (lane >= nb) ml[k] = make_float2(-INFINITY, 0.0f);
+                }
+                load(0);
+                float w[RPW]; // of this lane's split
+#pragma unroll
+                for (int k = 0; k < RPW; k++) {
+                    const float mn = fmaxf(M[k], wave_max(ml[k].x)), mr = mn == -INFINITY ? 0.0f : mn;
+                    const float sc = M[k] == -INFINITY ? 0.0f : softmax_exp2(M[k] - mr);
+                    w[k] = softmax_exp2(ml[k].x - mr);
+                    L[k] = L[k] * sc + wave_sum(w[k] * ml[k].y);
+#pragma unroll
+                    for (int e = 0; e < E; e++) O[k][e] *= sc;
+                    M[k] = mn;
+                }
+                for (uint32_t s = 0; s < nb; s += U) {
+                    float x[RPW][U][E];
+#pragma unroll
+                    for (int k = 0; k < RPW; k++)
+#pragma unroll
+                        for (int z = 0; z < U; z++)
+#pragma unroll
+                            for (int e = 0; e < E; e++) x[k][z][e] = v[k][z][e];
+                    if (s + U < nb) load(s + U);
+#pragma unroll
+                    for (int z = 0; z < U; z++) {
+                        if (s + z >= nb) break;
+#pragma unroll
+                        for (int k = 0; k < RPW; k++) {
+                            const float wt = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w[k]), s + z));
+#pragma unroll
+                            for (int e = 0; e < E; e++) O[k][e] = fmaf(x[k][z][e], wt, O[k][e]);
+                        }
+                    }
                 }
             }
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-            if (in) {
-                const size_t off = orow * a.ld_out + ohead * hs + d;
+#pragma unroll
+            for (int k = 0; k < RPW; k++) {
+                if (first + k >= rows || d >= hs) continue;
+                const float inv = L[k] == 0.0f ? 0.0f : 1.0f / L[k];
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    if constexpr (T == PA_H) ((uint16_t *)a.out)[off + e] = f32_to_f16(O[e] * inv);
-                    else ((float *)a.out)[off + e] = O[e] * inv;
+                    if constexpr (T == PA_H) ((uint16_t *)a.out)[out[k] + e] = f32_to_f16(O[k][e] * inv);
+                    else ((float *)a.out)[out[k] + e] = O[k][e] * inv;
                 }
             }
         }

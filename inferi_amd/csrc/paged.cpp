@@ -90,7 +90,6 @@ ifr_status launch_attention(ifr_ctx *c, PagedAttnArgs &a, const char *name, cons
                             uint32_t key_rows, uint32_t least, uint32_t most, uint32_t want, uint32_t max_kv) {
     const uint64_t base = tiles * a.n_sub * a.n_kv;
     if (!base) return IFR_OK;
-    if (base >= (1u << 23)) return c->fail(IFR_EUNSUPPORTED, "paged_attention: %llu workgroups", (unsigned long long)base);
     uint64_t keys = max_kv; // rows that a tile reads, at most
     if (a.window) keys = std::min<uint64_t>(keys, (uint64_t)a.window + a.sinks + a.QT + 2 * key_rows);
     const uint64_t key_tiles = (keys + key_rows - 1) / key_rows;
@@ -100,15 +99,20 @@ ifr_status launch_attention(ifr_ctx *c, PagedAttnArgs &a, const char *name, cons
     uint64_t splits = std::max<uint64_t>(1, std::min((key_tiles + chunk - 1) / chunk, PART_BYTES_MAX / row_bytes));
     a.chunk = (uint32_t)chunk;
     a.n_splits = (uint32_t)splits;
+    if (base * splits >= (1u << 24))
+        return c->fail(IFR_EUNSUPPORTED, "paged_attention: %llu workgroups", (unsigned long long)(base * splits));
     if (splits > 1) {
         if (ifr_status st = c->ensure_scratch(row_bytes * splits)) return st;
         a.part_o = (float *)c->scratch;
         a.part_ml = a.part_o + (uint64_t)a.n_rows * heads * splits * a.hs;
     }
-    ifr_status st = c->launch(name, dim3((uint32_t)base, a.n_splits), dim3(256), 0, a);
+    // (without a search a workgroup finds its split with its request)
+    const dim3 grid = a.search ? dim3((uint32_t)base, a.n_splits) : dim3((uint32_t)(base * splits));
+    ifr_status st = c->launch(name, grid, dim3(256), 0, a);
     if (st || splits == 1) return st;
-    // four rows of a tile per workgroup, one a wave
-    return c->launch(merge, dim3((uint32_t)base, (a.QT * a.heads_per + 3) / 4), dim3(256), 0, a);
+    // four waves a workgroup, of one row of a tile each (of four for the larger tiles)
+    const uint32_t rows = key_rows == 32 ? 4 : 16;
+    return c->launch(merge, dim3((uint32_t)base, (a.QT * a.heads_per + rows - 1) / rows), dim3(256), 0, a);
 }
 
 bool bad_ld(int64_t ld, int64_t least, int64_t unit) { return ld < least || ld % unit || ld > (1ll << 40); }

@@ -16,7 +16,7 @@ extern "C" __global__ void __launch_bounds__(PG_ROPE_THREADS) paged_rope_k(Paged
         pa_rows16_body<HSP, T>(a);                                                                          \
     }                                                                                                       \
     extern "C" __global__ void __launch_bounds__(256) paged_merge32_##NAME##_h##HSP(PagedAttnArgs a) {      \
-        pa_merge_body<HSP, T, PAD_KT>(a);                                                                   \
+        pa_merge_body<HSP, T, PAD_KT, 1>(a);                                                                \
     }
 
 PA_ROWS16(f16, 64, PA_H, 2)
@@ -26,16 +26,16 @@ PA_ROWS16(mixed, 128, PA_M, 2)
 PA_ROWS16(f32, 64, PA_S, 2)
 PA_ROWS16(f32, 128, PA_S, 2)
 
-#define PA_TILE(NAME, HSP, T, AHEAD)                                                                           \
+#define PA_TILE(NAME, HSP, T)                                                                                  \
     extern "C" __global__ void __launch_bounds__(64 * PAT_WAVES) __attribute__((amdgpu_waves_per_eu(2, 8))) \
     paged_tile_##NAME##_h##HSP(PagedAttnArgs a) {                                                           \
-        pa_tile_body<HSP, T, AHEAD>(a);                                                                     \
+        pa_tile_body<HSP, T>(a);                                                                            \
     }                                                                                                       \
     extern "C" __global__ void __launch_bounds__(256) paged_merge64_##NAME##_h##HSP(PagedAttnArgs a) {      \
-        pa_merge_body<HSP, T, PAT_KT>(a);                                                                   \
+        pa_merge_body<HSP, T, PAT_KT, 4>(a);                                                                \
     }
 
-PA_TILE(f16, 64, PA_H, 1)
-PA_TILE(f16, 128, PA_H, 1)
-PA_TILE(mixed, 64, PA_M, 1)
-PA_TILE(mixed, 128, PA_M, 0)
+PA_TILE(f16, 64, PA_H)
+PA_TILE(f16, 128, PA_H)
+PA_TILE(mixed, 64, PA_M)
+PA_TILE(mixed, 128, PA_M)
