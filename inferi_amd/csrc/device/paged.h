@@ -98,6 +98,8 @@ __device__ inline void paged_plan_body(const PagedPlanArgs &a) {
     __shared__ uint32_t s_start[PG_PLAN_THREADS + 1], s_off[PG_PLAN_THREADS], s_held[PG_PLAN_THREADS], s_kv[PG_PLAN_THREADS];
     const uint32_t tid = threadIdx.x, T = blockDim.x, pm = (1u << a.lp) - 1;
     const uint32_t cap = a.max_pages << a.lp; // at most 2^30
+    // the first round's lengths, read once for both passes
+    const uint32_t ctx0 = tid < a.n_requests ? a.ctx_len[tid] : 0, new0 = tid < a.n_requests ? a.new_len[tid] : 0;
     uint32_t top = min(*a.free_count, a.n_pages);
 
     // Released requests' pages onto the stack, those that are pages, in order:
@@ -107,29 +109,39 @@ __device__ inline void paged_plan_body(const PagedPlanArgs &a) {
     for (uint32_t base = 0; base < a.n_requests; base += T) {
         const uint32_t r = base + tid;
         uint32_t held = 0;
-        if (r < a.n_requests && a.new_len[r] == PG_RELEASE)
-            held = (uint32_t)min((uint64_t)a.max_pages, ((uint64_t)a.ctx_len[r] + pm) >> a.lp);
+        if (r < a.n_requests && (base ? a.new_len[r] : new0) == PG_RELEASE)
+            held = (uint32_t)min((uint64_t)a.max_pages, ((uint64_t)(base ? a.ctx_len[r] : ctx0) + pm) >> a.lp);
         if (!__syncthreads_or(held != 0)) continue;
         pushed = true;
-        uint32_t upto = held, none = 0, total, no;
-        block_scan2(upto, none, part, total, no);
-        s_start[tid] = upto - held;
+        // those that hold pages in a list: where each one's entries begin, and which it is (s_off, free until below)
+        uint32_t upto = held, listed = held != 0, total, n_listed, no;
+        block_scan2(upto, listed, part, total, n_listed);
+        if (held) {
+            s_start[listed - 1] = upto - held;
+            s_off[listed - 1] = r;
+        }
         __syncthreads();
-        for (uint32_t first = 0; first < total; first += 4 * T) {
-            uint32_t page[4], count = 0, zero = 0, all;
-            const uint32_t i0 = first + 4 * tid;
-            uint32_t j[4];
-            last_at_most_of(s_start, T, i0, j);
+        constexpr int N = 4;
+        for (uint32_t first = 0; first < total; first += N * T) {
+            uint32_t page[N], count = 0, zero = 0, all;
+            const uint32_t i0 = first + N * tid;
+            uint32_t j = i0 < total ? last_at_most(s_start, n_listed, i0) : 0;
 #pragma unroll
-            for (int z = 0; z < 4; z++)
-                page[z] = i0 + z < total ? a.table[(size_t)(base + j[z]) * a.max_pages + (i0 + z - s_start[j[z]])] : ~0u;
+            for (int z = 0; z < N; z++) {
+                page[z] = ~0u;
+                if (i0 + z < total) {
+                    // (each has an entry at least: the next entry is its own or the next one's first)
+                    if (z && j + 1 < n_listed && s_start[j + 1] <= i0 + z) j++;
+                    page[z] = a.table[(size_t)s_off[j] * a.max_pages + (i0 + z - s_start[j])];
+                }
+            }
 #pragma unroll
-            for (int z = 0; z < 4; z++) count += page[z] < a.n_pages;
+            for (int z = 0; z < N; z++) count += page[z] < a.n_pages;
             uint32_t to = count;
             block_scan2(to, zero, part, all, no);
             to += top - count;
 #pragma unroll
-            for (int z = 0; z < 4; z++)
+            for (int z = 0; z < N; z++)
                 if (page[z] < a.n_pages) {
                     if (to < a.n_pages) a.free_pages[to] = page[z];
                     to++;
@@ -145,7 +157,7 @@ __device__ inline void paged_plan_body(const PagedPlanArgs &a) {
     for (uint32_t base = 0; base < a.n_requests; base += T) {
         const uint32_t r = base + tid, nr = min(T, a.n_requests - base);
         const bool in = r < a.n_requests;
-        const uint32_t ctx = in ? a.ctx_len[r] : 0, nw = in ? a.new_len[r] : 0;
+        const uint32_t ctx = !base ? ctx0 : in ? a.ctx_len[r] : 0, nw = !base ? new0 : in ? a.new_len[r] : 0;
         const bool gone = nw == PG_RELEASE;
         // (one row past n_rows is as good as any more: the sums then stay exact up to there)
         const uint32_t n = gone ? 0 : min(nw, a.n_rows + 1), sum = gone ? ctx : add_sat(ctx, nw);
@@ -177,16 +189,21 @@ __device__ inline void paged_plan_body(const PagedPlanArgs &a) {
         if (ok && need) atomicMax(&s_fresh, off + need);
         __syncthreads();
         const uint32_t fresh = max(s_fresh, taken);
-        // the round's new table entries, four per thread and pass: popped page i is request j's, the last one
-        // whose pages begin at or before i (one without new pages shares its place with the next)
-        for (uint32_t i = taken + 4 * tid; i < fresh; i += 4 * T) {
-            uint32_t j[4];
-            last_at_most_of(s_off, nr, i, j);
+        // the round's new table entries: popped page i is request j's, the last one whose pages begin at or before
+        // i (one without new pages shares its place with the next)
+        auto entry = [&](uint32_t i, uint32_t j) {
+            a.table[(size_t)(base + j) * a.max_pages + s_held[j] + (i - s_off[j])] = a.free_pages[top - 1 - i];
+        };
+        if (fresh - taken <= T) {
+            if (taken + tid < fresh) entry(taken + tid, last_at_most(s_off, nr, taken + tid));
+        } else {
+            for (uint32_t i = taken + 4 * tid; i < fresh; i += 4 * T) {
+                uint32_t j[4];
+                last_at_most_of(s_off, nr, i, j);
 #pragma unroll
-            for (int z = 0; z < 4; z++)
-                if (i + z < fresh)
-                    a.table[(size_t)(base + j[z]) * a.max_pages + s_held[j[z]] + (i + z - s_off[j[z]])] =
-                        a.free_pages[top - 1 - i - z];
+                for (int z = 0; z < 4; z++)
+                    if (i + z < fresh) entry(i + z, j[z]);
+            }
         }
         if (a.rows_here) {
             const uint32_t first = s_start[0], last = base + nr == a.n_requests ? a.n_rows : s_start[nr];
@@ -222,7 +239,7 @@ __device__ inline void paged_rows_body(const PagedPlanArgs &a) {
     const uint32_t tid = threadIdx.x, row0 = blockIdx.x * PG_ROWS_PER;
     // the last request that starts at or before row0 (requests without rows
     // share their start with the next: the last one of them has row0)
-    uint32_t lo = 0, hi = a.n_requests;
+    uint32_t lo = 0, hi = a.n_requests <= PG_ROWS_WIN ? 1 : a.n_requests; // (all in the window: from the first)
     while (hi - lo > 1) {
         const uint32_t step = (hi - lo + 255) / 256, i = lo + tid * step;
         if (tid == 0) s_n = 0;

@@ -59,6 +59,12 @@ IFR_DEV uint32_t pa_entry(const uint32_t *p, uint32_t i) {
     return ((const_u32 *)(uintptr_t)p)[i];
 }
 
+// An address that all lanes share, in scalar registers.
+IFR_DEV const char *pa_scalar(const char *p) {
+    const uint64_t x = (uint64_t)p;
+    return (const char *)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32 |
+                          (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)x));
+}
 // Rows and cache length of request r, whatever the buffers hold.
 IFR_DEV void pa_request(const PagedAttnArgs &a, uint32_t r, uint32_t &row0, uint32_t &n, uint32_t &kv) {
     row0 = min(a.row_start[r], a.n_rows);
@@ -109,6 +115,14 @@ IFR_DEV bool pa_pick(uint32_t mine, uint32_t left, uint32_t &src, uint32_t &befo
 IFR_DEV bool pa_find(const PagedAttnArgs &a, uint32_t at, uint32_t &r, uint32_t &q0) {
     const uint32_t lane = threadIdx.x & 63;
     uint32_t src = 0, before = 0;
+    if (a.n_requests == 1) {
+        uint32_t row0, n, kv;
+        pa_request_uniform(a, 0, row0, n, kv);
+        const uint32_t nt = (n + a.QT - 1) / a.QT;
+        r = 0;
+        q0 = (nt - 1 - at) * a.QT;
+        return at < nt;
+    }
     if (a.n_requests <= 64) {
         uint32_t row0, n = 0, kv = 0, nt = 0;
         if (lane < a.n_requests) {
@@ -727,6 +741,7 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
         const char *p = (const char *)from + 2 * ((int64_t)(page < a.n_pages ? page : 0u) * a.page_stride +
                                                   (int64_t)((kt * PAT_KT + 16 * wave) & pm) * a.row_stride +
                                                   (int64_t)kvh * a.head_stride);
+        p = pa_scalar(p);
         const uint32_t lds = lds_addr(to) + b * TB + 16 * wave * RB;
 #pragma unroll
         for (uint32_t i = 0; i < 16 / LPI; i++) {

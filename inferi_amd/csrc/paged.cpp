@@ -153,7 +153,8 @@ IFR_API ifr_status ifr_paged_plan(ifr_ctx *c, const ifr_paged_plan_args *p) {
     a.lp = log2_of(p->page_size);
     a.max_pages = p->max_pages;
     a.rows_here = p->n_rows <= 2048 || !p->n_requests;
-    const uint32_t threads = p->n_requests <= 256 && p->n_rows <= 256 ? 256 : PG_PLAN_THREADS;
+    const uint32_t widest = std::max(p->n_requests, a.rows_here ? p->n_rows : 0u);
+    const uint32_t threads = widest <= 64 ? 64 : widest <= 256 ? 256 : PG_PLAN_THREADS;
     ifr_status st = c->launch("paged_plan_k", dim3(1), dim3(threads), 0, a);
     if (st || a.rows_here) return st;
     return c->launch("paged_rows_k", dim3((p->n_rows + 511) / 512), dim3(256), 0, a);

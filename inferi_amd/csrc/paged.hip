@@ -26,8 +26,8 @@ PA_ROWS16(mixed, 128, PA_M, 2)
 PA_ROWS16(f32, 64, PA_S, 2)
 PA_ROWS16(f32, 128, PA_S, 2)
 
-#define PA_TILE(NAME, HSP, T)                                                                                  \
-    extern "C" __global__ void __launch_bounds__(64 * PAT_WAVES) __attribute__((amdgpu_waves_per_eu(2, 8))) \
+#define PA_TILE(NAME, HSP, T, WPE)                                                                             \
+    extern "C" __global__ void __launch_bounds__(64 * PAT_WAVES) __attribute__((amdgpu_waves_per_eu(WPE, 8))) \
     paged_tile_##NAME##_h##HSP(PagedAttnArgs a) {                                                           \
         pa_tile_body<HSP, T>(a);                                                                            \
     }                                                                                                       \
@@ -35,7 +35,7 @@ PA_ROWS16(f32, 128, PA_S, 2)
         pa_merge_body<HSP, T, PAT_KT, 4>(a);                                                                \
     }
 
-PA_TILE(f16, 64, PA_H)
-PA_TILE(f16, 128, PA_H)
-PA_TILE(mixed, 64, PA_M)
-PA_TILE(mixed, 128, PA_M)
+PA_TILE(f16, 64, PA_H, 3)
+PA_TILE(f16, 128, PA_H, 2)
+PA_TILE(mixed, 64, PA_M, 2)
+PA_TILE(mixed, 128, PA_M, 2)
