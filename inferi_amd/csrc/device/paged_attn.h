@@ -37,6 +37,10 @@ struct PaTile {
 struct PaKeys {
     uint32_t ns, lo, n;
 };
+// Weights are 2^(s - r + 7): the largest that the reference lets through, 2^15,
+// is an f16 number still, and f16's smallest normal one is 2^-21 of a row's largest
+// weight.  (The factor is in the sums and the weighted rows alike.)
+constexpr float PA_UP = 7.0f;
 template <int KT>
 IFR_DEV PaKeys pa_keys(const PagedAttnArgs &a, const PaTile &t) {
     PaKeys k = {0, 0, 0};
@@ -235,6 +239,20 @@ IFR_DEV float pa_at(const void *p, size_t i) {
 IFR_DEV void pa_split(float x, _Float16 &hi, _Float16 &lo) {
     hi = (_Float16)x;
     lo = (_Float16)(x - (float)hi);
+}
+
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+// two f32 to a pair of f16, to nearest
+IFR_DEV uint32_t pa_pack(float x, float y) { return __builtin_bit_cast(uint32_t, half2v{(_Float16)x, (_Float16)y}); }
+// acc + both halves of a pair
+IFR_DEV float pa_add2(uint32_t h, float acc) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, h), half2v{(_Float16)1, (_Float16)1}, acc, false);
+}
+// x and y in two f16 parts each: the first 11 bits of each cut off, which is exact, and the rest rounded
+IFR_DEV void pa_split2(float x, float y, uint32_t &hi, uint32_t &lo) {
+    const float xh = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u), yh = __uint_as_float(__float_as_uint(y) & 0xFFFFE000u);
+    hi = pa_pack(xh, yh);
+    lo = pa_pack(x - xh, y - yh);
 }
 
 IFR_DEV bool pa_odd(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; } // infinite or NaN
@@ -494,8 +512,7 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) mt = fmaxf(mt, s[u][e]);
                 mt = pa_max4(mt);
-                // the reference moves only where a row's maximum passes it by more than 8: the weights stay
-                // below 2^8 (f16 holds them as well as those below 1) and most tiles rescale nothing
+                // the reference moves only where a row's maximum passes it by more than 8: most tiles rescale nothing
                 if (__ballot(mt > m + 8.0f)) {
                     const float mn = fmaxf(m, mt), al = mn == -INFINITY ? 0.0f : softmax_exp2(m - mn);
                     m = mn;
@@ -505,7 +522,7 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
 #pragma unroll
                         for (int e = 0; e < 4; e++) o[d][e] *= al;
                 }
-                const float mr = m == -INFINITY ? 0.0f : m;
+                const float mr = m == -INFINITY ? 0.0f : m - PA_UP;
                 float p[8];
 #pragma unroll
                 for (int u = 0; u < 2; u++)
@@ -521,14 +538,15 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                         for (int d = 0; d < DV; d++)
                             o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.v[j][d]), p[j], o[d], 0, 0, 0);
                 } else {
-                    half8v ph, pl;
+                    uint32_t hi[4], lo[4];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        _Float16 hi, lo;
-                        pa_split(p[j], hi, lo);
-                        ph[j] = hi;
-                        pl[j] = lo;
+                    for (int j = 0; j < 8; j += 2) {
+                        if constexpr (T == PA_M) pa_split2(p[j], p[j + 1], hi[j / 2], lo[j / 2]);
+                        else hi[j / 2] = pa_pack(p[j], p[j + 1]);
                     }
+                    const half8v ph = __builtin_bit_cast(half8v, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+                    half8v pl;
+                    if constexpr (T == PA_M) pl = __builtin_bit_cast(half8v, make_uint4(lo[0], lo[1], lo[2], lo[3]));
 #pragma unroll
                     for (int d = 0; d < DV; d++) {
                         // halves d of the eight rows' loads: the low or high half of word d / 2
@@ -573,7 +591,7 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                     const float s1 = pa_sum4(d4) * a.scale2;
                     if (!((int32_t)key <= qpos & ((int32_t)key > qlow | (int32_t)key < sinks))) continue;
                     const float mn = fmaxf(m, s1), mr = mn == -INFINITY ? 0.0f : mn;
-                    const float al = m == -INFINITY ? 0.0f : softmax_exp2(m - mr), p = softmax_exp2(s1 - mr);
+                    const float al = m == -INFINITY ? 0.0f : softmax_exp2(m - mr), p = softmax_exp2(s1 - mr + PA_UP);
                     m = mn;
                     // (0 x inf: a sum that was infinite stays so, or was NaN)
                     l = l * al + p;
@@ -735,7 +753,15 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
     auto page_of = [&](uint32_t kt) {
         return pa_entry(tab, min((kt * 4 + wave) >> (a.lp - 4), a.max_pages - 1));
     };
-    const uint32_t dma_row = lane / CPR, dma_chunk = lane % CPR;
+    // this lane's bytes of a load instruction, from its 16 rows' first (chunks past the head size: the last one,
+    // which meets q's zeros or outputs that nobody stores)
+    uint32_t k_off[16 / LPI], v_off[16 / LPI];
+#pragma unroll
+    for (uint32_t i = 0; i < 16 / LPI; i++) {
+        const uint32_t y = i * LPI + lane / CPR, c = lane % CPR;
+        k_off[i] = 2 * (y * (uint32_t)a.row_stride + 8 * min(c ^ kx(y), hs / 8 - 1));
+        v_off[i] = 2 * (y * (uint32_t)a.row_stride + 8 * min(c ^ vx(y), hs / 8 - 1));
+    }
     // this wave's 16 rows of tile kt into buffer b
     auto bring = [&](const void *from, char *to, uint32_t b, uint32_t kt, uint32_t page, bool k) {
         const char *p = (const char *)from + 2 * ((int64_t)(page < a.n_pages ? page : 0u) * a.page_stride +
@@ -744,12 +770,7 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
         p = pa_scalar(p);
         const uint32_t lds = lds_addr(to) + b * TB + 16 * wave * RB;
 #pragma unroll
-        for (uint32_t i = 0; i < 16 / LPI; i++) {
-            const uint32_t y = i * LPI + dma_row; // of the 16
-            // (chunks past the head size: the last one, which meets q's zeros or outputs that nobody stores)
-            const uint32_t c = min(dma_chunk ^ (k ? kx(y) : vx(y)), hs / 8 - 1);
-            lds_dma16(p, 2 * (y * (uint32_t)a.row_stride + 8 * c), lds + i * 1024);
-        }
+        for (uint32_t i = 0; i < 16 / LPI; i++) lds_dma16(p, k ? k_off[i] : v_off[i], lds + i * 1024);
     };
     uint32_t k_at[KC], v_at[DT]; // byte offsets of this lane's operands in a tile
 #pragma unroll
@@ -762,16 +783,17 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
     }
     auto scores = [&](uint32_t b, float16v (&s)[KB]) {
 #pragma unroll
-        for (int u = 0; u < KB; u++) {
+        for (int u = 0; u < KB; u++)
 #pragma unroll
             for (int e = 0; e < 16; e++) s[u][e] = 0.0f;
 #pragma unroll
-            for (int c = 0; c < KC; c++) {
+        for (int c = 0; c < KC; c++)
+#pragma unroll
+            for (int u = 0; u < KB; u++) {
                 const half8v av = *(const half8v *)(ks + b * TB + 32 * u * RB + k_at[c]);
                 s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, qh[c], s[u], 0, 0, 0);
                 if constexpr (T == PA_M) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, ql[c], s[u], 0, 0, 0);
             }
-        }
     };
     // V^T operand of 16 keys: block u, half cc, dims 32 d ..
     auto v_of = [&](uint32_t b, int u, int cc, int d) {
@@ -854,16 +876,27 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) o[d][e] *= al;
         }
-        const float mr = m == -INFINITY ? 0.0f : m;
+        const float mr = m == -INFINITY ? 0.0f : m - PA_UP;
         half8v ph[KB][2], pl[T == PA_M ? KB : 1][2];
 #pragma unroll
         for (int u = 0; u < KB; u++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const float p = softmax_exp2(fmaf(s[u][e], rs, -mr));
-                l += p;
-                ph[u][e / 8][e % 8] = (_Float16)p;
-                if constexpr (T == PA_M) pl[u][e / 8][e % 8] = (_Float16)(p - (float)ph[u][e / 8][e % 8]);
+            for (int cc = 0; cc < 2; cc++) {
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const float p0 = softmax_exp2(fmaf(s[u][8 * cc + e], rs, -mr)), p1 = softmax_exp2(fmaf(s[u][8 * cc + e + 1], rs, -mr));
+                    if constexpr (T == PA_M) {
+                        pa_split2(p0, p1, hi[e / 2], lo[e / 2]);
+                        l += p0 + p1;
+                    } else {
+                        // summed as they are multiplied: rounded
+                        hi[e / 2] = pa_pack(p0, p1);
+                        l = pa_add2(hi[e / 2], l);
+                    }
+                }
+                ph[u][cc] = __builtin_bit_cast(half8v, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+                if constexpr (T == PA_M) pl[u][cc] = __builtin_bit_cast(half8v, make_uint4(lo[0], lo[1], lo[2], lo[3]));
             }
 #pragma unroll
         for (int u = 0; u < KB; u++)
@@ -923,7 +956,7 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
                 const float s1 = (d2 + __shfl_xor(d2, 32, 64)) * a.scale2;
                 if (!((int32_t)key <= qpos & ((int32_t)key > qlow | (int32_t)key < sinks))) continue;
                 const float mn = fmaxf(m, s1), mr = mn == -INFINITY ? 0.0f : mn;
-                const float al = m == -INFINITY ? 0.0f : softmax_exp2(m - mr), p = softmax_exp2(s1 - mr);
+                const float al = m == -INFINITY ? 0.0f : softmax_exp2(m - mr), p = softmax_exp2(s1 - mr + PA_UP);
                 m = mn;
                 l = l * al + p;
 #pragma unroll
