@@ -241,6 +241,20 @@ IFR_DEV void pa_split(float x, _Float16 &hi, _Float16 &lo) {
     lo = (_Float16)(x - (float)hi);
 }
 
+// Asks the scheduler for LEAD operands' LDS reads (READS each), then a product and the
+// next operand's reads in turn, N operands in all (PRODUCTS each).  Left to itself
+// it keeps one read ahead, and every product waits out most of the LDS latency.
+template <int LEAD, int N, int PRODUCTS, int READS>
+IFR_DEV void pa_interleave() {
+    __builtin_amdgcn_sched_group_barrier(0x100, LEAD * READS, 0);
+#pragma unroll
+    for (int i = 0; i < N - LEAD; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x8, PRODUCTS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, LEAD * PRODUCTS, 0);
+}
+
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 // two f32 to a pair of f16, to nearest
 IFR_DEV uint32_t pa_pack(float x, float y) { return __builtin_bit_cast(uint32_t, half2v{(_Float16)x, (_Float16)y}); }
@@ -698,6 +712,51 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
     const size_t gq = t.row0 + (row_ok ? qi : 0);
     const uint32_t *tab = a.table + (size_t)r * a.max_pages;
 
+    // Chunk c of row y of a tile lies at chunk c ^ kx(y) (V: vx(y)) of the row.
+    // K's operand reads take the same chunk of 16 consecutive rows, V's four
+    // chunks (64 bytes) of four rows.
+    auto kx = [](uint32_t y) { return HSP == 128 ? y & 15 : (y >> 1) & 7; };
+    auto vx = [](uint32_t y) { return HSP == 128 ? 4 * (y & 3) : 4 * ((y >> 1) & 1); };
+    auto tile_of = [&](uint32_t i) {
+        i = min(i, i1 - 1);
+        return i < keys.ns ? i : keys.lo + i - keys.ns;
+    };
+    // the page of this wave's rows of tile kt
+    auto page_of = [&](uint32_t kt) {
+        return pa_entry(tab, min((kt * 4 + wave) >> (a.lp - 4), a.max_pages - 1));
+    };
+    // this lane's bytes of a load instruction, from its 16 rows' first (chunks past the head size: the last one,
+    // which meets q's zeros or outputs that nobody stores)
+    uint32_t k_off[16 / LPI], v_off[16 / LPI];
+#pragma unroll
+    for (uint32_t i = 0; i < 16 / LPI; i++) {
+        const uint32_t y = i * LPI + lane / CPR, c = lane % CPR;
+        k_off[i] = 2 * (y * (uint32_t)a.row_stride + 8 * min(c ^ kx(y), hs / 8 - 1));
+        v_off[i] = 2 * (y * (uint32_t)a.row_stride + 8 * min(c ^ vx(y), hs / 8 - 1));
+    }
+    // this wave's 16 rows of tile kt into buffer b
+    const int64_t head_off = 2 * (int64_t)kvh * a.head_stride;
+    auto bring = [&](uint32_t b, uint32_t kt, uint32_t page) {
+        const int64_t off = 2 * ((int64_t)(page < a.n_pages ? page : 0u) * a.page_stride +
+                                 (int64_t)((kt * PAT_KT + 16 * wave) & pm) * a.row_stride) + head_off;
+        const char *pk = pa_scalar((const char *)a.key + off), *pv = pa_scalar((const char *)a.value + off);
+        const uint32_t lds = b * TB + 16 * wave * RB;
+#pragma unroll
+        for (uint32_t i = 0; i < 16 / LPI; i++) lds_dma16(pk, k_off[i], lds_addr(ks) + lds + i * 1024);
+#pragma unroll
+        for (uint32_t i = 0; i < 16 / LPI; i++) lds_dma16(pv, v_off[i], lds_addr(vs) + lds + i * 1024);
+    };
+    if (tid < 3) s_flags[tid] = 0;
+    // The first tile on its way before the queries are read.  Tiles i and i + 1, and the latter's page:
+    uint32_t flag = 0, kt = 0, kt1 = 0, pg = 0, pg1 = 0;
+    if (i0 < i1) {
+        kt = tile_of(i0);
+        kt1 = tile_of(i0 + 1);
+        pg = page_of(kt);
+        pg1 = page_of(kt1);
+        bring(0, kt, pg);
+    }
+
     half8v qh[KC], ql[T == PA_M ? KC : 1];
     float rs = a.scale2;
     {
@@ -740,38 +799,6 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
         }
     }
 
-    // Chunk c of row y of a tile lies at chunk c ^ kx(y) (V: vx(y)) of the row.
-    // K's operand reads take the same chunk of 16 consecutive rows, V's four
-    // chunks (64 bytes) of four rows.
-    auto kx = [](uint32_t y) { return HSP == 128 ? y & 15 : (y >> 1) & 7; };
-    auto vx = [](uint32_t y) { return HSP == 128 ? 4 * (y & 3) : 4 * ((y >> 1) & 1); };
-    auto tile_of = [&](uint32_t i) {
-        i = min(i, i1 - 1);
-        return i < keys.ns ? i : keys.lo + i - keys.ns;
-    };
-    // the page of this wave's rows of tile kt
-    auto page_of = [&](uint32_t kt) {
-        return pa_entry(tab, min((kt * 4 + wave) >> (a.lp - 4), a.max_pages - 1));
-    };
-    // this lane's bytes of a load instruction, from its 16 rows' first (chunks past the head size: the last one,
-    // which meets q's zeros or outputs that nobody stores)
-    uint32_t k_off[16 / LPI], v_off[16 / LPI];
-#pragma unroll
-    for (uint32_t i = 0; i < 16 / LPI; i++) {
-        const uint32_t y = i * LPI + lane / CPR, c = lane % CPR;
-        k_off[i] = 2 * (y * (uint32_t)a.row_stride + 8 * min(c ^ kx(y), hs / 8 - 1));
-        v_off[i] = 2 * (y * (uint32_t)a.row_stride + 8 * min(c ^ vx(y), hs / 8 - 1));
-    }
-    // this wave's 16 rows of tile kt into buffer b
-    auto bring = [&](const void *from, char *to, uint32_t b, uint32_t kt, uint32_t page, bool k) {
-        const char *p = (const char *)from + 2 * ((int64_t)(page < a.n_pages ? page : 0u) * a.page_stride +
-                                                  (int64_t)((kt * PAT_KT + 16 * wave) & pm) * a.row_stride +
-                                                  (int64_t)kvh * a.head_stride);
-        p = pa_scalar(p);
-        const uint32_t lds = lds_addr(to) + b * TB + 16 * wave * RB;
-#pragma unroll
-        for (uint32_t i = 0; i < 16 / LPI; i++) lds_dma16(p, k ? k_off[i] : v_off[i], lds + i * 1024);
-    };
     uint32_t k_at[KC], v_at[DT]; // byte offsets of this lane's operands in a tile
 #pragma unroll
     for (int c = 0; c < KC; c++) k_at[c] = li * RB + 16 * ((2 * c + hl) ^ kx(li));
@@ -816,19 +843,18 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
         l = 0.0f;
     };
     clear();
-    if (tid < 3) s_flags[tid] = 0;
 
-    uint32_t flag = 0, kt = 0, kt1 = 0, pg1 = 0; // tiles i and i + 1, and the latter's page
     auto step = [&](uint32_t i, const uint32_t b) { // tile i, in buffer b
         float16v s[KB];
         const uint32_t k0 = kt * PAT_KT, nf = flag == 2 ? 0 : flag + 1;
         // (past the last tile: the last again, unused)
-        bring(a.key, ks, b ^ 1u, kt1, pg1, true);
-        bring(a.value, vs, b ^ 1u, kt1, pg1, false);
+        bring(b ^ 1u, kt1, pg1);
         const uint32_t kt2 = tile_of(i + 2), pg2 = page_of(kt2);
         const uint32_t f = __builtin_amdgcn_readfirstlane(s_flags[flag]);
         if (pg1 >= a.n_pages && lane == 0) atomicOr(&s_flags[nf], 1u << wave);
         scores(b, s);
+        // the operand reads run four ahead of the products that take them
+        pa_interleave<4, KB * KC, T == PA_M ? 2 : 1, 1>();
         // (uniform) keys past a row's position, or on no page; keys before a row's window
         const bool past = f || (int32_t)(k0 + PAT_KT - 1) > t.p0;
         const bool behind = a.window && (int64_t)k0 <= (int64_t)t.plast - a.window;
@@ -908,6 +934,7 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, ph[u][cc], o[d], 0, 0, 0);
                     if constexpr (T == PA_M) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, pl[u][cc], o[d], 0, 0, 0);
                 }
+        pa_interleave<4, KB * 2 * DT, T == PA_M ? 2 : 1, 2>();
         if (tid == 0) s_flags[nf == 2 ? 0 : nf + 1] = 0;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the rows brought above
         __syncthreads();
@@ -917,12 +944,6 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
         pg1 = pg2;
     };
     if (i0 < i1) {
-        kt = tile_of(i0);
-        kt1 = tile_of(i0 + 1);
-        const uint32_t pg = page_of(kt);
-        pg1 = page_of(kt1);
-        bring(a.key, ks, 0, kt, pg, true);
-        bring(a.value, vs, 0, kt, pg, false);
         __syncthreads(); // the flags are cleared
         if (pg >= a.n_pages && lane == 0) atomicOr(&s_flags[0], 1u << wave);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
