@@ -215,9 +215,10 @@ IFR_DEV uint32_t lds_addr(const void *p) { return (uint32_t)(uintptr_t)(const ld
 // The address is a wave-uniform base plus this lane's 32-bit byte offset.
 // M0 is reserved by the compiler (it sets M0 itself before each of its own
 // uses and ignores a clobber entry for it); the compiler-generated code of
-// these kernels does not read M0.
+// these kernels does not read M0.  A load into LDS needs one wait state after
+// the write of M0, which the compiler does not add inside assembly.
 IFR_DEV void lds_dma16(const void *base, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds));
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds));
 }
 
 // splitmix64 finaliser: a bijective 64-bit mix.
