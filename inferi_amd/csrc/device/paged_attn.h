@@ -262,11 +262,16 @@ IFR_DEV uint32_t pa_pack(float x, float y) { return __builtin_bit_cast(uint32_t,
 IFR_DEV float pa_add2(uint32_t h, float acc) {
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, h), half2v{(_Float16)1, (_Float16)1}, acc, false);
 }
-// x and y in two f16 parts each: the first 11 bits of each cut off, which is exact, and the rest rounded
+// x and y in two f16 parts each: the second is x - hi, formed and rounded in one
+// mixed-precision multiply-add.  (The pair and the -1 are hidden from the
+// compiler, which otherwise converts twice and back.)
 IFR_DEV void pa_split2(float x, float y, uint32_t &hi, uint32_t &lo) {
-    const float xh = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u), yh = __uint_as_float(__float_as_uint(y) & 0xFFFFE000u);
-    hi = pa_pack(xh, yh);
-    lo = pa_pack(x - xh, y - yh);
+    hi = pa_pack(x, y);
+    float minus = -1.0f;
+    asm("" : "+v"(hi));
+    asm("" : "+v"(minus));
+    const half2v h = __builtin_bit_cast(half2v, hi);
+    lo = __builtin_bit_cast(uint32_t, half2v{(_Float16)__builtin_fmaf((float)h[0], minus, x), (_Float16)__builtin_fmaf((float)h[1], minus, y)});
 }
 
 IFR_DEV bool pa_odd(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; } // infinite or NaN
