@@ -297,19 +297,24 @@ IFR_DEV int pa_q_exponent(float mx) { return mx > 0.0f && !pa_odd(mx) ? min(14 -
 //                 the lane (output row i of tile t is dim 8i + t).
 // So there is no LDS and no barrier in the loop; the waves' states are joined
 // through LDS once.  Rows whose page is no page read page 0 and are masked.
-constexpr int PAD_WAVES = 4, PAD_KT = 32, PAD_ROWS = 16;
+constexpr int PAD_WAVES = 4, PAD_ROWS = 16;
+// 16-row blocks of a key tile: two, which the f16 products' eight keys a lane
+// need; one for f32 rows of 128, whose two blocks do not fit the registers (54
+// spilled: 1191 rows over 1869 of 32 heads 379 us).
+template <int HSP, int T>
+constexpr int PAD_NU = T == PA_S && HSP == 128 ? 1 : 2;
 
 template <int HSP, int T>
 struct PaRegs {
     static constexpr int KC = T == PA_S ? HSP / 16 : HSP / 32; // 16-byte loads of a K row
     static constexpr int DV = HSP / 16;                        // dims of a V row per lane
-    uint4 k[2][KC];
-    uint32_t v[8][T == PA_S ? DV : DV / 2];
+    uint4 k[PAD_NU<HSP, T>][KC];
+    uint32_t v[4 * PAD_NU<HSP, T>][T == PA_S ? DV : DV / 2];
 };
 
 template <int HSP, int T>
 __device__ void pa_rows16_body(const PagedAttnArgs &a) {
-    constexpr int ES = T == PA_S ? 4 : 2, KC = PaRegs<HSP, T>::KC, DV = HSP / 16;
+    constexpr int ES = T == PA_S ? 4 : 2, KC = PaRegs<HSP, T>::KC, DV = HSP / 16, NU = PAD_NU<HSP, T>, PAD_KT = 16 * NU;
     constexpr int OP = HSP + 4;
     __shared__ __attribute__((aligned(16))) float og[PAD_WAVES][PAD_ROWS][OP];
     __shared__ float mg[PAD_WAVES][PAD_ROWS], lg[PAD_WAVES][PAD_ROWS];
@@ -358,7 +363,7 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
         };
         auto load_k = [&](uint32_t kt, uint32_t pg0, uint32_t pg1) {
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
+            for (int u = 0; u < NU; u++) {
                 const char *p = base_of(a.key, u ? pg1 : pg0, kt * PAD_KT + 16 * u);
                 const uint32_t off = n * (uint32_t)a.row_stride;
 #pragma unroll
@@ -370,7 +375,7 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
         };
         auto load_v = [&](uint32_t kt, uint32_t pg0, uint32_t pg1) {
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
+            for (int u = 0; u < NU; u++) {
                 const char *p = base_of(a.value, u ? pg1 : pg0, kt * PAD_KT + 16 * u);
                 const uint32_t d = min(dv, hs - DV);
 #pragma unroll
@@ -397,10 +402,10 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
         if (i0 + wave < i1) {
             kt = tile_of(i0 + wave);
             kn = tile_of(min(i0 + wave + PAD_WAVES, i1 - 1));
-            pg0 = page_of(2 * kt);
-            pg1 = page_of(2 * kt + 1);
-            pn0 = page_of(2 * kn);
-            pn1 = page_of(2 * kn + 1);
+            pg0 = page_of(NU * kt);
+            pg1 = page_of(NU * kt + 1);
+            pn0 = page_of(NU * kn);
+            pn1 = page_of(NU * kn + 1);
             load_k(kt, pg0, pg1);
             load_v(kt, pg0, pg1);
         }
@@ -470,14 +475,14 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                 const uint32_t k0 = kt * PAD_KT;
                 if (hs != HSP) { // (uniform) dims past the head size: zero, as q's are (0 x inf is not)
 #pragma unroll
-                    for (int u = 0; u < 2; u++)
+                    for (int u = 0; u < NU; u++)
 #pragma unroll
                         for (int c = 0; c < KC; c++)
                             if ((T == PA_S ? 16 : 32) * c + dk >= hs) x.k[u][c] = make_uint4(0, 0, 0, 0);
                 }
-                float4v s[2];
+                float4v s[NU];
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
+                for (int u = 0; u < NU; u++) {
                     s[u] = float4v{0, 0, 0, 0};
 #pragma unroll
                     for (int c = 0; c < KC; c++) {
@@ -494,17 +499,17 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                         }
                     }
                 }
-                const bool bad0 = pg0 >= a.n_pages, bad1 = pg1 >= a.n_pages;
+                const bool bad0 = pg0 >= a.n_pages, bad1 = NU == 2 && pg1 >= a.n_pages;
                 // the next tile's K (past the last: the last again, unused)
                 load_k(kn, pn0, pn1);
                 // (uniform) keys past a row's position, or on no page; keys before a row's window
                 const bool past = (int32_t)(k0 + PAD_KT - 1) > t.p0 || bad0 || bad1;
                 const bool behind = a.window && (int64_t)k0 <= (int64_t)t.plast - a.window;
 #pragma unroll
-                for (int u = 0; u < 2; u++) s[u] *= rs;
+                for (int u = 0; u < NU; u++) s[u] *= rs;
                 if (past) {
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
+                    for (int u = 0; u < NU; u++) {
                         const bool gone = u ? bad1 : bad0;
                         const int32_t first = (int32_t)(k0 + 16 * u + 4 * g);
                         const int32_t hi = (gone ? -1 : qpos) - first, thi = (gone ? -1 : t.plast) - first;
@@ -521,13 +526,13 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                 if (behind) {
                     const int32_t lo = qlow - (int32_t)(k0 + 4 * g), sk = sinks - (int32_t)(k0 + 4 * g);
 #pragma unroll
-                    for (int u = 0; u < 2; u++)
+                    for (int u = 0; u < NU; u++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) s[u][e] = (16 * u + e > lo) | (16 * u + e < sk) ? s[u][e] : -INFINITY;
                 }
                 float mt = -INFINITY;
 #pragma unroll
-                for (int u = 0; u < 2; u++)
+                for (int u = 0; u < NU; u++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) mt = fmaxf(mt, s[u][e]);
                 mt = pa_max4(mt);
@@ -542,9 +547,9 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                         for (int e = 0; e < 4; e++) o[d][e] *= al;
                 }
                 const float mr = m == -INFINITY ? 0.0f : m - PA_UP;
-                float p[8];
+                float p[4 * NU];
 #pragma unroll
-                for (int u = 0; u < 2; u++)
+                for (int u = 0; u < NU; u++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         p[4 * u + e] = softmax_exp2(s[u][e] - mr);
@@ -552,7 +557,7 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                     }
                 if constexpr (T == PA_S) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++)
+                    for (int j = 0; j < 4 * NU; j++)
 #pragma unroll
                         for (int d = 0; d < DV; d++)
                             o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.v[j][d]), p[j], o[d], 0, 0, 0);
@@ -585,8 +590,8 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                 pg0 = pn0;
                 pg1 = pn1;
                 kn = tile_of(min(i + 2 * PAD_WAVES, i1 - 1));
-                pn0 = page_of(2 * kn);
-                pn1 = page_of(2 * kn + 1);
+                pn0 = page_of(NU * kn);
+                pn1 = page_of(NU * kn + 1);
             }
         l = pa_sum4(l);
         // A weight of 0 times an infinity or NaN in a row of V that a query does not see is NaN (and the two parts
@@ -1015,7 +1020,7 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
     if (!one && hl == 0) *(float2 *)(a.part_ml + at * 2) = make_float2(m, l);
 }
 
-// Joins the splits of tiles of the 16-row kernel (KT 32, RPW 1) or of the tile
+// Joins the splits of tiles of the 16-row kernel (RPW 1) or of the tile
 // kernel (KT 64, RPW 4): grid as its x, and per y four waves of RPW rows of the
 // tile each.  A lane has the dims 2 lane, 2 lane + 1 (64 dims: one) of every
 // row, and one split's (m, l) of 64 at a time; the rows' loads go out together.

@@ -111,7 +111,7 @@ ifr_status launch_attention(ifr_ctx *c, PagedAttnArgs &a, const char *name, cons
     ifr_status st = c->launch(name, grid, dim3(256), 0, a);
     if (st || splits == 1) return st;
     // four waves a workgroup, of one row of a tile each (of four for the larger tiles)
-    const uint32_t rows = key_rows == 32 ? 4 : 16;
+    const uint32_t rows = key_rows == 64 ? 16 : 4;
     return c->launch(merge, dim3((uint32_t)base, (a.QT * a.heads_per + rows - 1) / rows), dim3(256), 0, a);
 }
 
@@ -290,8 +290,9 @@ IFR_API ifr_status ifr_paged_attention(ifr_ctx *c, const ifr_paged_cache *cache,
         a.search = max_new > QT16;
         const uint64_t tiles = a.search ? p->n_rows / a.QT + std::min(p->n_requests, p->n_rows) : p->n_requests;
         snprintf(name, sizeof name, "paged_rows16_%s_h%u", type, hsp);
-        snprintf(merge, sizeof merge, "paged_merge32_%s_h%u", type, hsp);
-        return launch_attention(c, a, name, merge, tiles, 32, PA_L16, PA_M16, PA_W16, max_kv);
+        snprintf(merge, sizeof merge, "paged_merge16_%s_h%u", type, hsp);
+        const uint32_t key_rows = k.dtype == IFR_F32 && hsp == 128 ? 16 : 32, per = 32 / key_rows; // (device/paged_attn.h PAD_NU)
+        return launch_attention(c, a, name, merge, tiles, key_rows, PA_L16 * per, PA_M16 * per, PA_W16, max_kv);
     }
     a.heads_per = a.G;
     a.n_sub = 1;
@@ -299,7 +300,7 @@ IFR_API ifr_status ifr_paged_attention(ifr_ctx *c, const ifr_paged_cache *cache,
     a.search = 1;
     const uint64_t tiles = p->n_rows / a.QT + std::min(p->n_requests, p->n_rows);
     snprintf(name, sizeof name, "paged_tile_%s_h%u", type, hsp);
-    snprintf(merge, sizeof merge, "paged_merge64_%s_h%u", type, hsp);
+    snprintf(merge, sizeof merge, "paged_merge128_%s_h%u", type, hsp);
     return launch_attention(c, a, name, merge, tiles, 64, PA_L128, PA_M128, PA_W128, max_kv);
 }
 

@@ -15,8 +15,8 @@ extern "C" __global__ void __launch_bounds__(PG_ROPE_THREADS) paged_rope_k(Paged
     paged_rows16_##NAME##_h##HSP(PagedAttnArgs a) {                                                         \
         pa_rows16_body<HSP, T>(a);                                                                          \
     }                                                                                                       \
-    extern "C" __global__ void __launch_bounds__(256) paged_merge32_##NAME##_h##HSP(PagedAttnArgs a) {      \
-        pa_merge_body<HSP, T, PAD_KT, 1>(a);                                                                \
+    extern "C" __global__ void __launch_bounds__(256) paged_merge16_##NAME##_h##HSP(PagedAttnArgs a) {      \
+        pa_merge_body<HSP, T, 16 * PAD_NU<HSP, T>, 1>(a);                                                   \
     }
 
 PA_ROWS16(f16, 64, PA_H, 2)
@@ -31,7 +31,7 @@ PA_ROWS16(f32, 128, PA_S, 2)
     paged_tile_##NAME##_h##HSP(PagedAttnArgs a) {                                                           \
         pa_tile_body<HSP, T>(a);                                                                            \
     }                                                                                                       \
-    extern "C" __global__ void __launch_bounds__(256) paged_merge64_##NAME##_h##HSP(PagedAttnArgs a) {      \
+    extern "C" __global__ void __launch_bounds__(256) paged_merge128_##NAME##_h##HSP(PagedAttnArgs a) {      \
         pa_merge_body<HSP, T, PAT_KT, 4>(a);                                                                \
     }
 
