@@ -273,55 +273,51 @@ __device__ inline void paged_rows_body(const PagedPlanArgs &a) {
 }
 
 // ------------------------------------------------------ RoPE and the store --
-// Workgroup (x, part): rows x * rows_per .., its part of their 8-element
-// items.  The angles' (cos, sin) of the rows go to LDS, one angle per thread:
-// theta_j = 2^(-2j/hs log2(base)) and pos * theta_j / 2pi in 64 bits, reduced
-// to a fraction of a turn there, cos and sin of it in f32 (at position 1e5 an
-// f32 product would be off by 4e-3).  An item is four pairs of one head: eight
-// contiguous elements, or four and the four half a head away (NeoX).  Memory
-// bound: each element is read once and written once.
-constexpr uint32_t PG_ROPE_LDS = 4 * 64; // (cos, sin) pairs: up to 4 rows of up to 64
+// Workgroup (row, part): the part's 8-element items of the row (one part where
+// the rows fill the chip).  The row's angles' (cos, sin) go to LDS, one angle
+// per thread: theta_j = 2^(-2j/hs log2(base)) and pos * theta_j / 2pi in 64
+// bits, reduced to a fraction of a turn there, cos and sin of it in f32 (at
+// position 1e5 an f32 product would be off by 4e-3).  An item is four pairs of
+// one head: eight contiguous elements, or four and the four half a head away
+// (NeoX).  Memory bound: each element is read once and written once.
+// 8190 rows of 48 heads of 128, f32 to an f16 cache: 58 us, 5.2 TB/s (in
+// workgroups of four rows, whose trigonometry fills their threads, 71: fewer of
+// them overlap their loads); 32 rows 4.3 us, with one workgroup a row 4.9.
+constexpr uint32_t PG_ROPE_LDS = 64; // (cos, sin) pairs of a row
 
 __device__ inline void paged_rope_body(const PagedRopeArgs &a) {
     __shared__ float2 cs[PG_ROPE_LDS];
-    __shared__ uint32_t s_pos[4];
-    __shared__ uint64_t s_slot[4];
     const uint32_t tid = threadIdx.x, hh = a.hs / 2, cpi = a.hs / 8;
-    const uint32_t row0 = blockIdx.x * a.rows_per, nrows = min(a.rows_per, a.n_rows - row0);
-    if (tid < nrows) {
-        s_pos[tid] = a.positions[row0 + tid];
-        s_slot[tid] = a.slots[row0 + tid];
-    }
-    for (uint32_t i = tid; i < nrows * hh; i += PG_ROPE_THREADS) {
-        const uint32_t m = i / hh, j = i % hh;
+    const size_t row = blockIdx.x;
+    const uint32_t pos = a.positions[row];
+    if (pos == PG_NO_ROW) return;
+    const uint64_t slot = a.slots[row], page = slot >> a.lp;
+    if (tid < hh) {
         float c = 1.0f, s = 0.0f;
         if (a.turn) {
-            const double th = exp2(-(double)(2 * j) / (double)a.hs * a.log2_base);
-            double t = (double)a.positions[row0 + m] * th * 0.15915494309189533577; // in turns
+            const double th = exp2(-(double)(2 * tid) / (double)a.hs * a.log2_base);
+            double t = (double)pos * th * 0.15915494309189533577; // in turns
             t -= rint(t);
             sincospif((float)(2.0 * t), &s, &c);
         }
-        cs[i] = make_float2(c, s);
+        cs[tid] = make_float2(c, s);
     }
     __syncthreads();
-    const uint32_t heads = (a.q ? a.n_heads : 0) + 2 * a.n_kv, per_row = heads * cpi;
-    const uint32_t items = nrows * per_row;
+    const uint32_t heads = (a.q ? a.n_heads : 0) + 2 * a.n_kv, items = heads * cpi;
     for (uint32_t it = blockIdx.y * PG_ROPE_THREADS + tid; it < items; it += a.parts * PG_ROPE_THREADS) {
-        const uint32_t m = it / per_row, w = it % per_row, h = w / cpi, ci = w % cpi;
-        if (s_pos[m] == PG_NO_ROW) continue;
+        const uint32_t h = it / cpi, ci = it % cpi;
         const uint32_t nq = heads - 2 * a.n_kv;
         const uint32_t what = h < nq ? 0u : h < nq + a.n_kv ? 1u : 2u; // q, k, v
         const uint32_t head = h - (what == 0 ? 0 : what == 1 ? nq : nq + a.n_kv);
         const bool pairs_apart = a.neox && what < 2;
         // the item's elements: e0 .. +4 and e1 .. +4 of the head
         const uint32_t e0 = pairs_apart ? 4 * ci : 8 * ci, e1 = pairs_apart ? e0 + hh : e0 + 4;
-        const size_t row = row0 + m;
         const float *x = (what == 0 ? a.q + row * a.ld_q : what == 1 ? a.k + row * a.ld_k : a.v + row * a.ld_v) +
                          (size_t)head * a.hs;
         const float4 u = *(const float4 *)(x + e0), v = *(const float4 *)(x + e1);
         float y[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
         if (what < 2 && a.turn) {
-            const float2 *ang = cs + m * hh + 4 * ci;
+            const float2 *ang = cs + 4 * ci;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int p = pairs_apart ? i : 2 * i, q = pairs_apart ? i + 4 : 2 * i + 1;
@@ -336,7 +332,6 @@ __device__ inline void paged_rope_body(const PagedRopeArgs &a) {
             f16 = a.q_f16;
             dst = (char *)a.q_out + (row * a.ld_q_out + (size_t)head * a.hs) * (f16 ? 2 : 4);
         } else {
-            const uint64_t slot = s_slot[m], page = slot >> a.lp;
             if (page >= a.n_pages) continue;
             f16 = a.kv_f16;
             const int64_t off = (int64_t)page * a.page_stride + (int64_t)(slot & ((1ull << a.lp) - 1)) * a.row_stride +

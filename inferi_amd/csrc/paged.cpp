@@ -11,31 +11,33 @@
 
 using namespace ifr;
 
-#ifndef PA_L16
-#define PA_L16 8
-#endif
-#ifndef PA_M16
-#define PA_M16 64
-#endif
-#ifndef PA_W16
-#define PA_W16 1024
-#endif
-#ifndef PA_FEW
-#define PA_FEW 2
-#endif
-#ifndef PA_L128
-#define PA_L128 4
-#endif
-#ifndef PA_M128
-#define PA_M128 1024
-#endif
-#ifndef PA_W128
-#define PA_W128 512
-#endif
 namespace {
 
 constexpr uint32_t MAX_CONTEXT = 1u << 30;          // max_pages * page_size, as max_pos
 constexpr uint64_t PART_BYTES_MAX = 512ull << 20;   // partials of one attention call
+constexpr uint64_t MAX_GRID = 1ull << 24;           // workgroups of 256 threads a launch takes
+
+// How the attention splits a call's keys over workgroups: chunks of as many key
+// tiles as make `want` workgroups if every tile of rows had the longest context,
+// `least` to `most` of them. Shorter chunks cost partials and a workgroup's fixed
+// 5 us, longer ones leave CUs idle or the last workgroups alone.
+struct Split { uint32_t key_rows, least, most, want; };
+
+// Tiles of 16 rows (measured on 256 CUs; us with the value below, at half and at
+// twice of it). least: one decode at 145 keys 5.8 / 8.7 / 5.9, 8 decodes of an f32
+// cache at up to 1000 13.6 / 16.1 / 15.6. most: 64 decodes at up to 4096 keys
+// 126 / 140 / 131, 55 of an f32 cache at 1719 205 / 273 / 204, but 12 at 1 to
+// 55745, where the longest alone remains, 27.6 / 22.3 / 27.5. want, at 512 / 768 /
+// 1024: 44 decodes in a window of 915 20.3 / 22.3 / 24.9, 43 f32 ones at 1 to
+// 4343 25.4 / 21.0 / 19.1, 64 at 2637 43.1 / 44.7 / 48.8.
+constexpr Split SPLIT16{32, 8, 64, 768};
+// The f32 rows of 128, whose key tiles are of 16: the same numbers of keys.
+constexpr Split SPLIT16_F32{16, 16, 128, 768};
+// Tiles of 128 rows. least: one chunk of 517 rows 31.1 / 31.2 / 33.2. most: 9
+// requests of 1 to 512 rows over 0 to 120000 keys 1497, 1655 at twice, 2229 without
+// a bound. want: three chunks of 200 rows over 2000 keys 61.4 / 54.5 / 65.7, 512
+// over 30000 285 / 383 / 293.
+constexpr Split SPLIT128{64, 4, 512, 512};
 
 uint32_t log2_of(uint32_t v) { return 31u - (uint32_t)__builtin_clz(v); }
 bool pow2(uint32_t v) { return v && !(v & (v - 1)); }
@@ -87,19 +89,19 @@ ifr_status check_cache(ifr_ctx *c, const char *who, ifr_paged_cache &k) {
 // tile; least, most: key tiles of a split (more only where a tile has more than
 // `most` of them for all its splits); want: workgroups that fill the chip.
 ifr_status launch_attention(ifr_ctx *c, PagedAttnArgs &a, const char *name, const char *merge, uint64_t tiles,
-                            uint32_t key_rows, uint32_t least, uint32_t most, uint32_t want, uint32_t max_kv) {
+                            const Split &by, uint32_t max_kv) {
     const uint64_t base = tiles * a.n_sub * a.n_kv;
     if (!base) return IFR_OK;
+    if (base >= MAX_GRID) return c->fail(IFR_EUNSUPPORTED, "paged_attention: %llu workgroups", (unsigned long long)base);
     uint64_t keys = max_kv; // rows that a tile reads, at most
-    if (a.window) keys = std::min<uint64_t>(keys, (uint64_t)a.window + a.sinks + a.QT + 2 * key_rows);
-    const uint64_t key_tiles = (keys + key_rows - 1) / key_rows;
+    if (a.window) keys = std::min<uint64_t>(keys, (uint64_t)a.window + a.sinks + a.QT + 2 * by.key_rows);
+    const uint64_t key_tiles = (keys + by.key_rows - 1) / by.key_rows;
     const uint64_t heads = (uint64_t)a.n_kv * a.G, row_bytes = (uint64_t)a.n_rows * heads * (a.hs + 2) * 4;
-    // chunks of the keys that make `want` workgroups if all tiles are as long as the longest may be
-    uint64_t chunk = std::max<uint64_t>(least, std::min<uint64_t>(most, key_tiles * base / want));
+    uint64_t chunk = std::max<uint64_t>(by.least, std::min<uint64_t>(by.most, key_tiles * base / by.want));
     uint64_t splits = std::max<uint64_t>(1, std::min((key_tiles + chunk - 1) / chunk, PART_BYTES_MAX / row_bytes));
     a.chunk = (uint32_t)chunk;
     a.n_splits = (uint32_t)splits;
-    if (base * splits >= (1u << 24))
+    if (base * splits >= MAX_GRID)
         return c->fail(IFR_EUNSUPPORTED, "paged_attention: %llu workgroups", (unsigned long long)(base * splits));
     if (splits > 1) {
         if (ifr_status st = c->ensure_scratch(row_bytes * splits)) return st;
@@ -111,7 +113,7 @@ ifr_status launch_attention(ifr_ctx *c, PagedAttnArgs &a, const char *name, cons
     ifr_status st = c->launch(name, grid, dim3(256), 0, a);
     if (st || splits == 1) return st;
     // four waves a workgroup, of one row of a tile each (of four for the larger tiles)
-    const uint32_t rows = key_rows == 64 ? 16 : 4;
+    const uint32_t rows = by.key_rows == 64 ? 16 : 4;
     return c->launch(merge, dim3((uint32_t)base, (a.QT * a.heads_per + rows - 1) / rows), dim3(256), 0, a);
 }
 
@@ -152,7 +154,8 @@ IFR_API ifr_status ifr_paged_plan(ifr_ctx *c, const ifr_paged_plan_args *p) {
     a.n_pages = p->n_pages;
     a.lp = log2_of(p->page_size);
     a.max_pages = p->max_pages;
-    a.rows_here = p->n_rows <= 2048 || !p->n_requests;
+    // (2048 rows by the plan's workgroup 4.9 us, by a second launch 7.4; 3074 6.0 and 7.5; 11274 11.9 and 11.3)
+    a.rows_here = p->n_rows <= 8192 || !p->n_requests;
     const uint32_t widest = std::max(p->n_requests, a.rows_here ? p->n_rows : 0u);
     const uint32_t threads = widest <= 64 ? 64 : widest <= 256 ? 256 : PG_PLAN_THREADS;
     ifr_status st = c->launch("paged_plan_k", dim3(1), dim3(threads), 0, a);
@@ -212,12 +215,12 @@ IFR_API ifr_status ifr_paged_rope_store(ifr_ctx *c, const ifr_paged_cache *cache
     a.neox = p->variant == IFR_ROPE_NEOX;
     a.q_f16 = p->q_dtype == IFR_F16;
     a.kv_f16 = k.dtype == IFR_F16;
-    a.rows_per = p->n_rows >= 4 * (uint32_t)c->n_cu ? 4 : 1;
+    // a workgroup a row, or several that share it while that leaves CUs without one
     const uint32_t items = ((p->q ? p->n_heads : 0) + 2 * k.n_kv_heads) * (hs / 8);
-    a.parts = a.rows_per > 1 ? 1 : std::max(1u, std::min((items + PG_ROPE_THREADS - 1) / PG_ROPE_THREADS,
-                                                         (uint32_t)c->n_cu * 2 / p->n_rows));
+    a.parts = std::max(1u, std::min((items + PG_ROPE_THREADS - 1) / PG_ROPE_THREADS, (uint32_t)c->n_cu * 2 / p->n_rows));
+    if (p->n_rows >= MAX_GRID) return c->fail(IFR_EUNSUPPORTED, "paged_rope_store: %u rows", p->n_rows);
     DeviceGuard dev(c->device);
-    return c->launch("paged_rope_k", dim3((p->n_rows + a.rows_per - 1) / a.rows_per, a.parts), dim3(PG_ROPE_THREADS), 0, a);
+    return c->launch("paged_rope_k", dim3(p->n_rows, a.parts), dim3(PG_ROPE_THREADS), 0, a);
 }
 
 IFR_API ifr_status ifr_paged_attention(ifr_ctx *c, const ifr_paged_cache *cache, const ifr_paged_attn_args *p) {
@@ -275,11 +278,16 @@ IFR_API ifr_status ifr_paged_attention(ifr_ctx *c, const ifr_paged_cache *cache,
     const uint32_t max_new = p->max_new ? std::min(p->max_new, p->n_rows) : p->n_rows;
     const uint32_t max_kv = p->max_kv ? std::min(p->max_kv, cap) : cap;
 
-    // Steps of up to `few` new rows a request run in tiles of 16 (query, head) rows,
-    // longer ones, with the decodes among them, in tiles of 128 (f32 caches, whose
-    // products run at a sixteenth of the rate and need no larger tile, and groups
-    // of more than 64 heads, always in the former).
-    const uint32_t QT16 = std::max(16 / a.G, 1u), few = PA_FEW * QT16;
+    // Steps of up to `few` new rows a request (two tiles of 16 (query, head) rows for
+    // heads of 64 and less, one for larger ones) run in such tiles, longer ones, with the
+    // decodes among them, in tiles of 128, which read K and V once for more rows. Two
+    // tiles' worth, us in tiles of 16 and of 128: heads of 128, 16 requests over 2000
+    // keys 48.8 / 40.9, 64 over 500 44.1 / 33.2, one over 30000 50 / 56; heads of 64, 64
+    // over 1000 25.6 / 26.1 and, with f32 rows, 25.8 / 30.4. Three tiles' worth: 12 rows
+    // of 4 requests over 9000 71.6 / 45.7. f32 caches (whose products run at a sixteenth
+    // of the rate and gain nothing from larger tiles) and groups of more than 64 heads
+    // (fewer than two rows of 128) always run in tiles of 16.
+    const uint32_t QT16 = std::max(16 / a.G, 1u), few = (hsp == 64 ? 2 : 1) * QT16;
     DeviceGuard dev(c->device);
     char name[64], merge[64];
     if (k.dtype == IFR_F32 || a.G > 64 || max_new <= few) {
@@ -291,8 +299,7 @@ IFR_API ifr_status ifr_paged_attention(ifr_ctx *c, const ifr_paged_cache *cache,
         const uint64_t tiles = a.search ? p->n_rows / a.QT + std::min(p->n_requests, p->n_rows) : p->n_requests;
         snprintf(name, sizeof name, "paged_rows16_%s_h%u", type, hsp);
         snprintf(merge, sizeof merge, "paged_merge16_%s_h%u", type, hsp);
-        const uint32_t key_rows = k.dtype == IFR_F32 && hsp == 128 ? 16 : 32, per = 32 / key_rows; // (device/paged_attn.h PAD_NU)
-        return launch_attention(c, a, name, merge, tiles, key_rows, PA_L16 * per, PA_M16 * per, PA_W16, max_kv);
+        return launch_attention(c, a, name, merge, tiles, k.dtype == IFR_F32 && hsp == 128 ? SPLIT16_F32 : SPLIT16, max_kv);
     }
     a.heads_per = a.G;
     a.n_sub = 1;
@@ -301,7 +308,7 @@ IFR_API ifr_status ifr_paged_attention(ifr_ctx *c, const ifr_paged_cache *cache,
     const uint64_t tiles = p->n_rows / a.QT + std::min(p->n_requests, p->n_rows);
     snprintf(name, sizeof name, "paged_tile_%s_h%u", type, hsp);
     snprintf(merge, sizeof merge, "paged_merge128_%s_h%u", type, hsp);
-    return launch_attention(c, a, name, merge, tiles, 64, PA_L128, PA_M128, PA_W128, max_kv);
+    return launch_attention(c, a, name, merge, tiles, SPLIT128, max_kv);
 }
 
 } // extern "C"

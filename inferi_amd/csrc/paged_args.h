@@ -29,7 +29,7 @@ struct PagedRopeArgs {
     double log2_base;
     uint32_t n_rows, n_heads, n_kv, hs, n_pages, lp;
     uint32_t neox, turn, q_f16, kv_f16;
-    uint32_t rows_per, parts; // rows of a workgroup; workgroups that share them
+    uint32_t parts; // workgroups that share a row
 };
 
 struct PagedAttnArgs {

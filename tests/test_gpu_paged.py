@@ -389,6 +389,17 @@ def test_bounds_only_size_the_launch(ctx, kind, max_new, max_kv):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("max_kv", [1, 300, 0])
+def test_unequal_decodes_past_the_bound(ctx, kind, max_kv):
+    """Decodes of very unequal lengths, most or all longer than the caller said: up to 64 and more requests."""
+    rng = np.random.default_rng(19)
+    for n in (2, 40, 64, 70):
+        lens = [(int(c), 1) for c in np.exp(rng.uniform(0, np.log(2500), n))]
+        lens[n // 2] = (6000, 1)
+        check(*attn_case(ctx, rng, kind, 4, 2, 64, 16, lens, max_kv=max_kv))
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_values_far_from_one(ctx, kind):
     """Large scores (one row carries all), tiny and huge query rows, a scale of the caller's."""
     rng = np.random.default_rng(15)
