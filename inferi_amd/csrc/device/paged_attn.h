@@ -177,10 +177,12 @@ IFR_DEV bool pa_find(const PagedAttnArgs &a, uint32_t at, uint32_t &r, uint32_t 
     return false;
 }
 
-// Key tiles of each split of request r's tiles, where a workgroup serves them all: by its last tile's keys.
+// Key tiles of each split of request r's tiles, where a workgroup serves them all: by its last tile's keys.  (Under
+// a window an earlier tile may have one more, as its ends fall, and one more as the last has fewer rows.)
 template <int KT>
 IFR_DEV uint32_t pa_request_chunk(const PagedAttnArgs &a, uint32_t r, uint32_t row0, uint32_t n, uint32_t kv, uint32_t &keys) {
     keys = pa_keys<KT>(a, pa_tile(a, r, row0, n, kv, n ? (n - 1) / a.QT * a.QT : 0)).n;
+    if (a.window && n > a.QT) keys += 2;
     return pa_chunk(a, keys);
 }
 // The `at`-th split of all requests, the longest first (whole chunks, then the

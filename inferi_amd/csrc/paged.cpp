@@ -26,7 +26,7 @@ struct Split { uint32_t key_rows, least, most, want; };
 // Tiles of 16 rows (measured on 256 CUs; us with the value below, at half and at
 // twice of it). least: one decode at 145 keys 5.8 / 8.7 / 5.9, 8 decodes of an f32
 // cache at up to 1000 13.6 / 16.1 / 15.6. most: 64 decodes at up to 4096 keys
-// 126 / 140 / 131, 55 of an f32 cache at 1719 205 / 273 / 204, but 12 at 1 to
+// 126 / 140 / 131, 1629 rows over 129 of an f32 cache 205 / 273 / 204, but 12 at 1 to
 // 55745, where the longest alone remains, 27.6 / 22.3 / 27.5. want, at 512 / 768 /
 // 1024: 44 decodes in a window of 915 20.3 / 22.3 / 24.9, 43 f32 ones at 1 to
 // 4343 25.4 / 21.0 / 19.1, 64 at 2637 43.1 / 44.7 / 48.8.

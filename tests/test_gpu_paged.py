@@ -400,6 +400,17 @@ def test_unequal_decodes_past_the_bound(ctx, kind, max_kv):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("requests", [1, 5, 66])
+def test_windows_with_more_rows_than_the_bound(ctx, kind, requests):
+    """Rows past max_new under a window of some whole chunks of keys: a request's earlier tiles reach over more key
+    tiles than its last one."""
+    rng = np.random.default_rng(20)
+    for window in (225, 240, 256, 481, 490, 497, 505, 512, 520):
+        lens = [(1000 + 13 * i, 9 + i % 40) if i < 5 else (3, 1) for i in range(requests)]
+        check(*attn_case(ctx, rng, kind, 4, 2, 64, 16, lens, window=window, sinks=window % 5, max_new=1))
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_values_far_from_one(ctx, kind):
     """Large scores (one row carries all), tiny and huge query rows, a scale of the caller's."""
     rng = np.random.default_rng(15)
