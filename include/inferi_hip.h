@@ -305,7 +305,8 @@ typedef struct {
  * IFR_NO_ROW and IFR_NO_SLOT for rows of a refused request and past the last
  * one.  A slot on an entry that is no page is IFR_NO_SLOT.
  * ctx_len_out may be ctx_len and free_count_out free_count; no other buffers
- * may overlap.  A page belongs to one request at a time. */
+ * may overlap.  A page belongs to one request at a time.  min(n_requests, 1024)
+ * rows of the table have fewer than 2^31 entries. */
 typedef struct {
     uint32_t n_requests, n_rows, n_pages, page_size, max_pages;
     const uint32_t *ctx_len, *new_len; /* device, [n_requests] */
@@ -334,7 +335,8 @@ IFR_API ifr_status ifr_paged_plan(ifr_ctx *ctx, const ifr_paged_plan_args *args)
  * out altogether; one whose slot is not in the cache stores nothing, but its
  * q is turned.  A slot that two rows share ends with one row's values, which
  * one is not said.  q, k, v 16-byte aligned, ld_q, ld_k, ld_v
- * multiples of 4, q_out 16-byte aligned with ld_q_out a multiple of 8. */
+ * multiples of 4, q_out 16-byte aligned with ld_q_out a multiple of 8; fewer
+ * than 2^24 rows. */
 typedef struct {
     uint32_t n_rows, n_heads;
     int32_t variant;

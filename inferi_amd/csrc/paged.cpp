@@ -99,10 +99,9 @@ ifr_status launch_attention(ifr_ctx *c, PagedAttnArgs &a, const char *name, cons
     const uint64_t heads = (uint64_t)a.n_kv * a.G, row_bytes = (uint64_t)a.n_rows * heads * (a.hs + 2) * 4;
     uint64_t chunk = std::max<uint64_t>(by.least, std::min<uint64_t>(by.most, key_tiles * base / by.want));
     uint64_t splits = std::max<uint64_t>(1, std::min((key_tiles + chunk - 1) / chunk, PART_BYTES_MAX / row_bytes));
+    splits = std::min(splits, (MAX_GRID - 1) / base);
     a.chunk = (uint32_t)chunk;
     a.n_splits = (uint32_t)splits;
-    if (base * splits >= MAX_GRID)
-        return c->fail(IFR_EUNSUPPORTED, "paged_attention: %llu workgroups", (unsigned long long)(base * splits));
     if (splits > 1) {
         if (ifr_status st = c->ensure_scratch(row_bytes * splits)) return st;
         a.part_o = (float *)c->scratch;

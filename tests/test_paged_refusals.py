@@ -127,5 +127,27 @@ def test_attention_refuses(host, kw):
 def test_attention_does_not_take(host):
     assert attn(host, dict(dtype=I.F32))[0] == EUNSUPPORTED       # f16 queries over an f32 cache
     assert "f16 queries" in attn(host, dict(dtype=I.F32))[1]
+    st, why = rope(host, n_rows=1 << 24)                           # a workgroup a row
+    assert st == EUNSUPPORTED and "rows" in why and "code object" not in why
     st, why = attn(host, n_requests=1 << 23, n_heads=2)            # more workgroups than one launch takes
     assert st == EUNSUPPORTED and "workgroups" in why
+
+
+@pytest.mark.parametrize("scale,ok", [(0.0, True), (2.0 ** -60, True), (2.0 ** 14, True), (2.0 ** -61, False), (1e-30, False),
+                                      (2.0 ** 14 * 1.001, False), (1e5, False), (-0.5, False)])
+def test_scales(host, scale, ok):
+    assert attn(host, scale=scale)[0] == (EUNSUPPORTED if ok else EINVAL)
+
+
+def test_plan_tables(host):
+    """Entries of 1024 requests are counted in 32 bits."""
+    assert plan(host, n_requests=31, max_pages=1 << 26)[0] == EUNSUPPORTED
+    assert plan(host, n_requests=32, max_pages=1 << 26)[0] == EINVAL
+    assert plan(host, n_requests=1 << 20, max_pages=(1 << 21) - 1)[0] == EUNSUPPORTED
+    assert plan(host, n_requests=1 << 20, max_pages=1 << 21)[0] == EINVAL
+
+
+def test_many_rows_over_long_tables(host):
+    """Launches of many tiles take fewer splits, not an error."""
+    assert "not in the code object" in attn(host, dict(page_size=1 << 20, max_pages=1 << 10), n_requests=1 << 20, n_rows=1 << 20,
+                                            max_kv=0)[1]
