@@ -74,7 +74,9 @@ typedef struct ifr_ctx ifr_ctx;
 
 /* Opens device `device`, creates the context's stream and loads the gfx950
  * code object (`code_object_path`, or NULL for inferi_kernels.hsaco beside
- * this library).  Replaces LlmOps::new (crates/inferi/src/context.rs:58-85),
+ * this library), and inferi_paged.hsaco from the same directory, or else from
+ * this library's (the ifr_paged_* kernels; without it only those calls fail).
+ * Replaces LlmOps::new (crates/inferi/src/context.rs:58-85),
  * which loads every compiled kernel of the backend. */
 IFR_API ifr_status ifr_create(int32_t device, const char *code_object_path, ifr_ctx **out);
 IFR_API void ifr_destroy(ifr_ctx *ctx);

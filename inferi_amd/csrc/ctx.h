@@ -86,7 +86,7 @@ struct ifr_ctx {
         // would set the thread's last HIP error, and clearing that one would
         // take away an error that the program itself left there
         hipModule_t from = name.compare(0, 6, "paged_") ? module : paged_module;
-        if (hipModuleGetFunction(&f, from, name.c_str()) != hipSuccess) f = nullptr;
+        if (from && hipModuleGetFunction(&f, from, name.c_str()) != hipSuccess) f = nullptr;
         fns[name] = f;
         return f;
     }

@@ -10,6 +10,7 @@
 // chat_llama2.rs:191-255), with the position, the token sequence and the
 // argmax all on the device.
 #include <dlfcn.h>
+#include <unistd.h>
 #include <hip/hip_runtime_api.h>
 
 #include <algorithm>
@@ -906,23 +907,24 @@ IFR_API ifr_status ifr_create(int32_t device, const char *code_object_path, ifr_
         return bail(c->fail(IFR_EUNSUPPORTED, "device %d is %s; this build targets gfx950", device, prop.gcnArchName));
     // default-priority stream (no priority argument anywhere)
     if ((st = c->hip(hipStreamCreateWithFlags(&c->stream, hipStreamNonBlocking), "hipStreamCreate"))) return bail(st);
+    Dl_info info;
+    const std::string library = dladdr((void *)&ifr_create, &info) && info.dli_fname ? info.dli_fname : "";
+    auto beside = [](const std::string &file, const char *name) {
+        const size_t slash = file.rfind('/');
+        return (slash == std::string::npos ? std::string(".") : file.substr(0, slash)) + "/" + name;
+    };
     std::string path;
-    if (code_object_path && *code_object_path) {
-        path = code_object_path;
-    } else {
-        Dl_info info;
-        if (!dladdr((void *)&ifr_create, &info) || !info.dli_fname)
-            return bail(c->fail(IFR_EINVAL, "cannot locate the library to find inferi_kernels.hsaco"));
-        path = info.dli_fname;
-        size_t slash = path.rfind('/');
-        path = (slash == std::string::npos ? std::string(".") : path.substr(0, slash)) + "/inferi_kernels.hsaco";
-    }
+    if (code_object_path && *code_object_path) path = code_object_path;
+    else if (!library.empty()) path = beside(library, "inferi_kernels.hsaco");
+    else return bail(c->fail(IFR_EINVAL, "cannot locate the library to find inferi_kernels.hsaco"));
     if ((st = c->hip(hipModuleLoad(&c->module, path.c_str()), ("hipModuleLoad(" + path + ")").c_str())))
         return bail(st);
-    // the paged-cache kernels lie beside it
-    const size_t dir = path.rfind('/');
-    const std::string paged = (dir == std::string::npos ? std::string() : path.substr(0, dir + 1)) + "inferi_paged.hsaco";
-    if ((st = c->hip(hipModuleLoad(&c->paged_module, paged.c_str()), ("hipModuleLoad(" + paged + ")").c_str())))
+    // The paged-cache kernels lie beside it, or beside the library.  (Whoever ships neither
+    // has every other operator; the paged ones then fail.)
+    std::string paged = beside(path, "inferi_paged.hsaco");
+    if (access(paged.c_str(), R_OK) && !library.empty()) paged = beside(library, "inferi_paged.hsaco");
+    if (!access(paged.c_str(), R_OK) &&
+        (st = c->hip(hipModuleLoad(&c->paged_module, paged.c_str()), ("hipModuleLoad(" + paged + ")").c_str())))
         return bail(st);
     for (auto &e : c->events)
         if ((st = c->hip(hipEventCreate(&e), "hipEventCreate"))) return bail(st);

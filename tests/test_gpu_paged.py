@@ -15,6 +15,8 @@ those below 2^-14 of the largest, at most n of them), so 2^-11 + n * 2^-25 of ma
 result's own rounding, 2^-11 of it.
 """
 
+import shutil
+
 import numpy as np
 import pytest
 
@@ -535,3 +537,17 @@ def test_serving_steps(ctx, kind, window):
     for y in (free, count, lens, table):
         y.free()
     cache.free()
+
+
+def test_code_object_without_the_paged_one_beside_it(tmp_path):
+    """A code object of the caller's in a directory of its own: the paged kernels then come from the library's."""
+    path = tmp_path / "kernels.hsaco"
+    shutil.copy(I.HSACO_PATH, path)
+    other = I.LlmContext(0, str(path))
+    a, b = other.upload(np.arange(8, dtype=np.float32)), other.upload(np.ones(8, np.float32))
+    other.add_assign(a, b, 8)
+    np.testing.assert_array_equal(a.download(), np.arange(8) + 1)
+    check(*attn_case(other, np.random.default_rng(21), "f16", 4, 2, 64, 16, [(20, 1), (0, 40)]))
+    a.free()
+    b.free()
+    other.close()
