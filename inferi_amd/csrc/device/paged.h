@@ -93,6 +93,7 @@ IFR_DEV void paged_row(const PagedPlanArgs &a, uint32_t row, uint32_t start, uin
 // latency of its chain: lengths, a scan, the popped pages with the pages of the
 // rows.  The rows take their pages from where they come from (the request's
 // last page, or the free list), not from the table entries written beside them.
+// 32 decodes 4.1 us, 1021 requests 13 (a launch that does nothing: 3.3).
 __device__ inline void paged_plan_body(const PagedPlanArgs &a) {
     __shared__ uint32_t part[32], s_fresh;
     __shared__ uint32_t s_start[PG_PLAN_THREADS + 1], s_off[PG_PLAN_THREADS], s_held[PG_PLAN_THREADS], s_kv[PG_PLAN_THREADS];
@@ -231,7 +232,8 @@ __device__ inline void paged_plan_body(const PagedPlanArgs &a) {
 
 // The rows of a large step, 256 threads each with rows of its own.  A
 // workgroup finds its first row's request by a 256-way search of row_start,
-// and its rows' among the next 1024 requests' starts in LDS.
+// and its rows' among the next 1024 requests' starts in LDS: 58885 rows of 1021
+// requests 5 us.
 constexpr uint32_t PG_ROWS_PER = 512, PG_ROWS_WIN = 1024;
 
 __device__ inline void paged_rows_body(const PagedPlanArgs &a) {

@@ -111,10 +111,10 @@ IFR_DEV bool pa_pick(uint32_t mine, uint32_t left, uint32_t &src, uint32_t &befo
     before = __builtin_amdgcn_readlane(sum - mine, src);
     return true;
 }
-// The `at`-th tile of all requests; false if there are
-// fewer.  Up to 64 requests, one a lane: the tiles in the order of their last
-// positions (by 64), the farthest first, so that the workgroups with the most
-// keys start first (nine requests' chunks, in the order of the requests 567 us).
+// The `at`-th tile of all requests; false if there are fewer.  Up to 64
+// requests, one a lane: the tiles in the order of their last positions (by 64),
+// the farthest first, so that the workgroups with the most keys start first
+// (nine requests' chunks 513 us, in the order of the requests 567).
 // More: from the last request's last tile, 64 requests a step.
 IFR_DEV bool pa_find(const PagedAttnArgs &a, uint32_t at, uint32_t &r, uint32_t &q0) {
     const uint32_t lane = threadIdx.x & 63;
@@ -188,7 +188,7 @@ IFR_DEV uint32_t pa_request_chunk(const PagedAttnArgs &a, uint32_t r, uint32_t r
 // The `at`-th split of all requests, the longest first (whole chunks, then the
 // requests' last parts by length): workgroups of unequal lengths, the long ones
 // started last, had left the chip half empty at the end (64 decodes of 200 to
-// 8191 rows 139 us).  More than 64 requests: split by split.
+// 8192 rows 125 us, in the order of the requests 139).  More than 64 requests: split by split.
 template <int KT>
 IFR_DEV bool pa_find_split(const PagedAttnArgs &a, uint32_t at, uint32_t &r, uint32_t &split) {
     const uint32_t R = a.n_requests, lane = threadIdx.x & 63;
@@ -299,6 +299,13 @@ IFR_DEV int pa_q_exponent(float mx) { return mx > 0.0f && !pa_odd(mx) ? min(14 -
 //                 the lane (output row i of tile t is dim 8i + t).
 // So there is no LDS and no barrier in the loop; the waves' states are joined
 // through LDS once.  Rows whose page is no page read page 0 and are masked.
+// Bound by memory where the keys are many: 64 decodes of 200 to 8192 rows, 8 KV
+// heads of 128 in f16, 125 us, 4.7 TB/s; two of 106 K and 131 K 190 us, 5.1
+// TB/s (a large copy: 4.8).  Both need the next key tile's loads in flight over
+// the products, which is 8 waves a CU by the registers; with 12 and 43
+// registers spilled the former is 205 us.  Short calls are a chain of trips to
+// memory: one decode of 145 rows 5.5 us.  f32 caches are bound by the f32
+// products: 1629 rows over 129 of 32 heads of 128, 205 us.
 constexpr int PAD_WAVES = 4, PAD_ROWS = 16;
 // 16-row blocks of a key tile: two, which the f16 products' eight keys a lane
 // need; one for f32 rows of 128, whose two blocks do not fit the registers (54
@@ -692,7 +699,14 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
 // the row, so that the operand reads fall on distinct banks; V^T's operands
 // are read with the transposing LDS load (lane i of 16 gets column i of four
 // rows of 16).  Wave w brings the tile's rows 16w .. 16w + 15, which lie on
-// one page.
+// one page.  Bound by the matrix products, the softmax beside them and power:
+// 5720 rows of nine requests over 306 to 8000, 32 heads of 128, 492 GFLOP in
+// 513 us, 0.96 PFLOP/s with the matrix pipes 42-47% busy (a library's f16
+// product of 8192^3: 1.14).  Scores one key tile ahead of the softmax took fewer
+// cycles but as long (the clock fell from 2.0 to 1.7 GHz); one buffer of V and
+// three workgroups a CU 592 us.  Of f32 rows, whose products are done twice and
+// whose weights are split on the vector units, 517 over 1021, 32 heads of 64: 22
+// us, and the merge 8.
 constexpr int PAT_WAVES = 4, PAT_ROWS = 32 * PAT_WAVES, PAT_KT = 64;
 
 template <int HSP, int T>
@@ -1028,7 +1042,9 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
 // row, and one split's (m, l) of 64 at a time; the rows' loads go out together.
 // Bound by the latency of its chain (request, (m, l) with the first partials,
 // output) and then by the partials' bytes.  Only splits that the tile has are
-// read; a tile of one split is written already.
+// read; a tile of one split is written already.  8 decodes in up to 24 splits:
+// 4 us.  (A launch of its own: the kernel boundary orders the partials, and the
+// one-sequence decode's merge by the last workgroup to arrive measured slower.)
 template <int HSP, int T, int KT, int RPW>
 __device__ void pa_merge_body(const PagedAttnArgs &a) {
     constexpr int E = HSP / 64, U = RPW == 1 ? 16 : 4; // U: partials of a row on their way

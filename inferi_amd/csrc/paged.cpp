@@ -25,7 +25,7 @@ struct Split { uint32_t key_rows, least, most, want; };
 
 // Tiles of 16 rows (measured on 256 CUs; us with the value below, at half and at
 // twice of it). least: one decode at 145 keys 5.8 / 8.7 / 5.9, 8 decodes of an f32
-// cache at up to 1000 13.6 / 16.1 / 15.6. most: 64 decodes at up to 4096 keys
+// cache at 1110 to 6000 13.6 / 16.1 / 15.6. most: 64 decodes at 200 to 8192 keys
 // 126 / 140 / 131, 1629 rows over 129 of an f32 cache 205 / 273 / 204, but 12 at 1 to
 // 55745, where the longest alone remains, 27.6 / 22.3 / 27.5. want, at 512 / 768 /
 // 1024: 44 decodes in a window of 915 20.3 / 22.3 / 24.9, 43 f32 ones at 1 to
@@ -33,7 +33,7 @@ struct Split { uint32_t key_rows, least, most, want; };
 constexpr Split SPLIT16{32, 8, 64, 768};
 // The f32 rows of 128, whose key tiles are of 16: the same numbers of keys.
 constexpr Split SPLIT16_F32{16, 16, 128, 768};
-// Tiles of 128 rows. least: one chunk of 517 rows 31.1 / 31.2 / 33.2. most: 9
+// Tiles of 128 rows. least: a chunk of 517 rows over 1021 31.1 / 31.2 / 33.2. most: 9
 // requests of 1 to 512 rows over 0 to 120000 keys 1497, 1655 at twice, 2229 without
 // a bound. want: three chunks of 200 rows over 2000 keys 61.4 / 54.5 / 65.7, 512
 // over 30000 285 / 383 / 293.

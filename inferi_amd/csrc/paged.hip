@@ -10,21 +10,22 @@ extern "C" __global__ void __launch_bounds__(PG_PLAN_THREADS) paged_plan_k(Paged
 extern "C" __global__ void __launch_bounds__(256) paged_rows_k(PagedPlanArgs a) { paged_rows_body(a); }
 extern "C" __global__ void __launch_bounds__(PG_ROPE_THREADS) paged_rope_k(PagedRopeArgs a) { paged_rope_body(a); }
 
-#define PA_ROWS16(NAME, HSP, T, WPE)                                                                        \
-    extern "C" __global__ void __launch_bounds__(64 * PAD_WAVES) __attribute__((amdgpu_waves_per_eu(WPE, 8))) \
-    paged_rows16_##NAME##_h##HSP(PagedAttnArgs a) {                                                         \
-        pa_rows16_body<HSP, T>(a);                                                                          \
-    }                                                                                                       \
-    extern "C" __global__ void __launch_bounds__(256) paged_merge16_##NAME##_h##HSP(PagedAttnArgs a) {      \
-        pa_merge_body<HSP, T, 16 * PAD_NU<HSP, T>, 1>(a);                                                   \
+// (two waves per SIMD: the registers of the next key tile's rows)
+#define PA_ROWS16(NAME, HSP, T)                                                                           \
+    extern "C" __global__ void __launch_bounds__(64 * PAD_WAVES) __attribute__((amdgpu_waves_per_eu(2, 8))) \
+    paged_rows16_##NAME##_h##HSP(PagedAttnArgs a) {                                                       \
+        pa_rows16_body<HSP, T>(a);                                                                        \
+    }                                                                                                     \
+    extern "C" __global__ void __launch_bounds__(256) paged_merge16_##NAME##_h##HSP(PagedAttnArgs a) {    \
+        pa_merge_body<HSP, T, 16 * PAD_NU<HSP, T>, 1>(a);                                                 \
     }
 
-PA_ROWS16(f16, 64, PA_H, 2)
-PA_ROWS16(f16, 128, PA_H, 2)
-PA_ROWS16(mixed, 64, PA_M, 2)
-PA_ROWS16(mixed, 128, PA_M, 2)
-PA_ROWS16(f32, 64, PA_S, 2)
-PA_ROWS16(f32, 128, PA_S, 2)
+PA_ROWS16(f16, 64, PA_H)
+PA_ROWS16(f16, 128, PA_H)
+PA_ROWS16(mixed, 64, PA_M)
+PA_ROWS16(mixed, 128, PA_M)
+PA_ROWS16(f32, 64, PA_S)
+PA_ROWS16(f32, 128, PA_S)
 
 #define PA_TILE(NAME, HSP, T, WPE)                                                                             \
     extern "C" __global__ void __launch_bounds__(64 * PAT_WAVES) __attribute__((amdgpu_waves_per_eu(WPE, 8))) \
