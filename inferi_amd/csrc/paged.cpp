@@ -21,7 +21,7 @@ constexpr uint64_t MAX_GRID = 1ull << 24;           // workgroups of 256 threads
 // tiles as make `want` workgroups if every tile of rows had the longest context,
 // `least` to `most` of them. Shorter chunks cost partials and a workgroup's fixed
 // 5 us, longer ones leave CUs idle or the last workgroups alone.
-struct Split { uint32_t key_rows, least, most, want; };
+struct Split { uint32_t key_rows, least, most, want; }; // (want 0: split128)
 
 // Tiles of 16 rows (measured on 256 CUs; us with the value below, at half and at
 // twice of it). least: one decode at 145 keys 5.8 / 8.7 / 5.9, 8 decodes of an f32
@@ -33,11 +33,33 @@ struct Split { uint32_t key_rows, least, most, want; };
 constexpr Split SPLIT16{32, 8, 64, 768};
 // The f32 rows of 128, whose key tiles are of 16: the same numbers of keys.
 constexpr Split SPLIT16_F32{16, 16, 128, 768};
-// Tiles of 128 rows. least: a chunk of 517 rows over 1021 31.1 / 31.2 / 33.2. most: 9
-// requests of 1 to 512 rows over 0 to 120000 keys 1497, 1655 at twice, 2229 without
-// a bound. want: three chunks of 200 rows over 2000 keys 61.4 / 54.5 / 65.7, 512
-// over 30000 285 / 383 / 293.
-constexpr Split SPLIT128{64, 4, 512, 512};
+// Tiles of 128 rows, whose chunks split128 finds. most: 9 requests of 1 to 512 rows
+// over 0 to 120000 keys 1497, 1655 at twice, 2229 without a bound.
+constexpr Split SPLIT128{64, 4, 512, 0};
+
+// Chunk of a call of `base` tiles of 128 rows over up to n key tiles. A key tile takes
+// a workgroup 1.15 us alone on its CU, two that share one 1.3 times as long; the join
+// takes 8 us and 5 ns a workgroup for its partials. The S parts that cost least by that
+// (us, S as chosen / another): 1024 rows of 32 heads of 128 over 4096, window 1024, 1
+// part 30 / 2 parts 43; 512 over 2000 4 parts 41 / 1 part 54; 512 over 30000 4 parts
+// 276 / 1 part 562; 2048 of 12 heads over 4096 3 parts 92 / 1 part 117. Chunks for 512
+// workgroups whatever n, and at least 4 key tiles: 1024 rows over none 36 (1 part: 27).
+uint64_t split128(uint64_t base, uint64_t n, uint32_t n_cu) {
+    uint64_t best = n;
+    double least = 0.0;
+    for (uint64_t parts = 1; parts <= n; parts++) {
+        const uint64_t chunk = (n + parts - 1) / parts, groups = base * parts;
+        if (parts > 1 && (chunk < SPLIT128.least || groups > 8 * n_cu)) break;
+        const double cus = (double)groups / n_cu; // workgroups a CU
+        const double step = cus <= 1.0 ? 1.0 : cus <= 2.0 ? 1.0 + 0.3 * (cus - 1.0) : 1.3 * cus / 2.0;
+        const double us = 1.15 * step * (double)chunk + (parts > 1 ? 8.0 + 0.005 * (double)groups : 0.0);
+        if (parts == 1 || us < least) {
+            least = us;
+            best = chunk;
+        }
+    }
+    return best;
+}
 
 uint32_t log2_of(uint32_t v) { return 31u - (uint32_t)__builtin_clz(v); }
 bool pow2(uint32_t v) { return v && !(v & (v - 1)); }
@@ -97,7 +119,8 @@ ifr_status launch_attention(ifr_ctx *c, PagedAttnArgs &a, const char *name, cons
     if (a.window) keys = std::min<uint64_t>(keys, (uint64_t)a.window + a.sinks + a.QT + 2 * by.key_rows);
     const uint64_t key_tiles = (keys + by.key_rows - 1) / by.key_rows;
     const uint64_t heads = (uint64_t)a.n_kv * a.G, row_bytes = (uint64_t)a.n_rows * heads * (a.hs + 2) * 4;
-    uint64_t chunk = std::max<uint64_t>(by.least, std::min<uint64_t>(by.most, key_tiles * base / by.want));
+    const uint64_t ideal = by.want ? key_tiles * base / by.want : split128(base, key_tiles, c->n_cu);
+    const uint64_t chunk = std::max<uint64_t>(by.least, std::min<uint64_t>(by.most, ideal));
     uint64_t splits = std::max<uint64_t>(1, std::min((key_tiles + chunk - 1) / chunk, PART_BYTES_MAX / row_bytes));
     splits = std::min(splits, (MAX_GRID - 1) / base);
     a.chunk = (uint32_t)chunk;
