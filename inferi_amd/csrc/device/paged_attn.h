@@ -209,15 +209,24 @@ IFR_DEV bool pa_find_split(const PagedAttnArgs &a, uint32_t at, uint32_t &r, uin
         split = at - before;
         return true;
     }
-    const uint32_t k = at - (uint32_t)__builtin_amdgcn_readlane(pa_wave_sum(full), 63);
-    uint32_t rank = 0;
-    for (uint32_t j = 0; j < R; j++) {
-        const uint32_t other = __builtin_amdgcn_readlane(rest, j);
-        rank += (other > rest) | ((other == rest) & (j < lane));
+    // the k-th largest of the last parts, bit by bit from the top (a comparison of each with all took 2.5 us of 64
+    // requests' 14); equal ones in the order of the requests
+    uint32_t k = at - (uint32_t)__builtin_amdgcn_readlane(pa_wave_sum(full), 63);
+    uint64_t left = __ballot(rest);
+    if ((uint32_t)__popcll(left) <= k) return false;
+    uint32_t most = a.chunk + 1; // (a chunk is longer where the splits would not reach)
+    while (__ballot(rest > most)) most *= 2;
+    for (int bit = 31 - __builtin_clz(most); bit >= 0; bit--) {
+        const uint64_t ones = left & __ballot(rest >> bit & 1u);
+        const uint32_t c = (uint32_t)__popcll(ones);
+        if (k < c) left = ones;
+        else {
+            k -= c;
+            left &= ~ones;
+        }
     }
-    const uint64_t is = __ballot(rest && rank == k);
-    if (!is) return false;
-    r = __builtin_amdgcn_readfirstlane((uint32_t)__ffsll((unsigned long long)is) - 1);
+    const uint32_t ahead = __builtin_amdgcn_mbcnt_hi((uint32_t)(left >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)left, 0));
+    r = (uint32_t)__ffsll((unsigned long long)(left & __ballot(ahead == k))) - 1;
     split = __builtin_amdgcn_readlane(full, r);
     return true;
 }

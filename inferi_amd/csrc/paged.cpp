@@ -17,39 +17,40 @@ constexpr uint32_t MAX_CONTEXT = 1u << 30;          // max_pages * page_size, as
 constexpr uint64_t PART_BYTES_MAX = 512ull << 20;   // partials of one attention call
 constexpr uint64_t MAX_GRID = 1ull << 24;           // workgroups of 256 threads a launch takes
 
-// How the attention splits a call's keys over workgroups: chunks of as many key
-// tiles as make `want` workgroups if every tile of rows had the longest context,
-// `least` to `most` of them. Shorter chunks cost partials and a workgroup's fixed
-// 5 us, longer ones leave CUs idle or the last workgroups alone.
-struct Split { uint32_t key_rows, least, most, want; }; // (want 0: split128)
+// How the attention splits a call's keys over workgroups (measured on 256 CUs, times in
+// us): of `base` tiles over up to n key tiles each, the key tiles of a part.
 
-// Tiles of 16 rows (measured on 256 CUs; us with the value below, at half and at
-// twice of it). least: one decode at 145 keys 5.8 / 8.7 / 5.9, 8 decodes of an f32
-// cache at 1110 to 6000 13.6 / 16.1 / 15.6. most: 64 decodes at 200 to 8192 keys
-// 126 / 140 / 131, 1629 rows over 129 of an f32 cache 205 / 273 / 204, but 12 at 1 to
-// 55745, where the longest alone remains, 27.6 / 22.3 / 27.5. want, at 512 / 768 /
-// 1024: 44 decodes in a window of 915 20.3 / 22.3 / 24.9, 43 f32 ones at 1 to
-// 4343 25.4 / 21.0 / 19.1, 64 at 2637 43.1 / 44.7 / 48.8.
-constexpr Split SPLIT16{32, 8, 64, 768};
-// The f32 rows of 128, whose key tiles are of 16: the same numbers of keys.
-constexpr Split SPLIT16_F32{16, 16, 128, 768};
-// Tiles of 128 rows, whose chunks split128 finds. most: 9 requests of 1 to 512 rows
-// over 0 to 120000 keys 1497, 1655 at twice, 2229 without a bound.
-constexpr Split SPLIT128{64, 4, 512, 0};
+// Tiles of 16 rows, n key tiles of 32; four waves take turns at them. A part costs a
+// workgroup's fixed 5 us, its partials and the second launch 4 more, so up to 16 stay
+// whole (one decode at 300 keys 6.2, in two 9.1). From half as many tiles as CUs the
+// memory is busy with 32 each (16 / 32 / 64 decodes of 1000, 32 heads over 8 of 128:
+// 16.5 / 29.5 / 53.9, in parts of 8 19.2 / 38.6 / 62.8); fewer tiles take parts down to
+// 8 (8 decodes of 300 to 1000 keys of an f32 cache 13.6, of 4 16.1, of 16 15.6), as many
+// as there are places for (two a CU: one over 16000 keys 19 to 21, in more 30; two over
+// 64000 108, in 784 parts 117, in 1008 119). Beyond 64 the longest sequences remain
+// alone at the end (64 decodes at 200 to 8192 126, parts of 32 140, of 128 131).
+uint64_t split16(uint64_t base, uint64_t n, uint32_t n_cu) {
+    if (n <= 16) return n;
+    const uint64_t places = 2 * n_cu;
+    return std::max<uint64_t>(2 * base >= n_cu ? 32 : 8, std::min<uint64_t>(64, (n * base + places - 1) / places));
+}
 
-// Chunk of a call of `base` tiles of 128 rows over up to n key tiles. A key tile takes
-// a workgroup 1.15 us alone on its CU, two that share one 1.3 times as long; the join
-// takes 8 us and 5 ns a workgroup for its partials. The S parts that cost least by that
-// (us, S as chosen / another): 1024 rows of 32 heads of 128 over 4096, window 1024, 1
-// part 30 / 2 parts 43; 512 over 2000 4 parts 41 / 1 part 54; 512 over 30000 4 parts
-// 276 / 1 part 562; 2048 of 12 heads over 4096 3 parts 92 / 1 part 117. Chunks for 512
-// workgroups whatever n, and at least 4 key tiles: 1024 rows over none 36 (1 part: 27).
+// Tiles of 128 rows, n key tiles of 64. A key tile takes a workgroup 1.15 us alone on its
+// CU, two that share one 1.3 times as long; the join takes 8 us and 5 ns a workgroup for
+// its partials. The number of parts that costs least by that, of those that all have
+// places (`base` counts up to a tile a request too many). As chosen / another, us: 1024
+// rows of 32 heads of 128 over 4096, window 1024, 1 part 30 / 2 parts 43; 512 over 2000
+// 4 parts 41 / 1 part 54; 512 over 30000 4 parts 276 / 1 part 562; 2048 of 12 heads over
+// 4096 2 parts 95 / 1 part 117; 517 of 32 heads of 64 over 1021, f32 over f16, 4 parts 30
+// / 5 parts, not all with places, 34. Parts for 512 workgroups whatever n: 1024 rows over
+// none 36 (1 part: 27). At most 512 key tiles, whatever that costs: 9 requests of 1 to
+// 512 rows over 0 to 120000 keys 1497, 1024 1655, no bound 2229.
 uint64_t split128(uint64_t base, uint64_t n, uint32_t n_cu) {
     uint64_t best = n;
     double least = 0.0;
     for (uint64_t parts = 1; parts <= n; parts++) {
         const uint64_t chunk = (n + parts - 1) / parts, groups = base * parts;
-        if (parts > 1 && (chunk < SPLIT128.least || groups > 8 * n_cu)) break;
+        if (parts > 1 && (chunk < 4 || 8 * groups > 17 * n_cu)) break;
         const double cus = (double)groups / n_cu; // workgroups a CU
         const double step = cus <= 1.0 ? 1.0 : cus <= 2.0 ? 1.0 + 0.3 * (cus - 1.0) : 1.3 * cus / 2.0;
         const double us = 1.15 * step * (double)chunk + (parts > 1 ? 8.0 + 0.005 * (double)groups : 0.0);
@@ -58,7 +59,7 @@ uint64_t split128(uint64_t base, uint64_t n, uint32_t n_cu) {
             best = chunk;
         }
     }
-    return best;
+    return std::min<uint64_t>(best, 512);
 }
 
 uint32_t log2_of(uint32_t v) { return 31u - (uint32_t)__builtin_clz(v); }
@@ -111,16 +112,18 @@ ifr_status check_cache(ifr_ctx *c, const char *who, ifr_paged_cache &k) {
 // tile; least, most: key tiles of a split (more only where a tile has more than
 // `most` of them for all its splits); want: workgroups that fill the chip.
 ifr_status launch_attention(ifr_ctx *c, PagedAttnArgs &a, const char *name, const char *merge, uint64_t tiles,
-                            const Split &by, uint32_t max_kv) {
+                            uint32_t key_rows, uint32_t max_kv) {
     const uint64_t base = tiles * a.n_sub * a.n_kv;
     if (!base) return IFR_OK;
     if (base >= MAX_GRID) return c->fail(IFR_EUNSUPPORTED, "paged_attention: %llu workgroups", (unsigned long long)base);
     uint64_t keys = max_kv; // rows that a tile reads, at most
-    if (a.window) keys = std::min<uint64_t>(keys, (uint64_t)a.window + a.sinks + a.QT + 2 * by.key_rows);
-    const uint64_t key_tiles = (keys + by.key_rows - 1) / by.key_rows;
+    if (a.window) keys = std::min<uint64_t>(keys, (uint64_t)a.window + a.sinks + a.QT + 2 * key_rows);
+    const uint64_t key_tiles = (keys + key_rows - 1) / key_rows;
     const uint64_t heads = (uint64_t)a.n_kv * a.G, row_bytes = (uint64_t)a.n_rows * heads * (a.hs + 2) * 4;
-    const uint64_t ideal = by.want ? key_tiles * base / by.want : split128(base, key_tiles, c->n_cu);
-    const uint64_t chunk = std::max<uint64_t>(by.least, std::min<uint64_t>(by.most, ideal));
+    // (key tiles of 16, of f32 rows of 128: as many keys)
+    const uint64_t chunk = key_rows == 64   ? split128(base, key_tiles, c->n_cu)
+                           : key_rows == 32 ? split16(base, key_tiles, c->n_cu)
+                                            : 2 * split16(base, (key_tiles + 1) / 2, c->n_cu);
     uint64_t splits = std::max<uint64_t>(1, std::min((key_tiles + chunk - 1) / chunk, PART_BYTES_MAX / row_bytes));
     splits = std::min(splits, (MAX_GRID - 1) / base);
     a.chunk = (uint32_t)chunk;
@@ -135,7 +138,7 @@ ifr_status launch_attention(ifr_ctx *c, PagedAttnArgs &a, const char *name, cons
     ifr_status st = c->launch(name, grid, dim3(256), 0, a);
     if (st || splits == 1) return st;
     // four waves a workgroup, of one row of a tile each (of four for the larger tiles)
-    const uint32_t rows = by.key_rows == 64 ? 16 : 4;
+    const uint32_t rows = key_rows == 64 ? 16 : 4;
     return c->launch(merge, dim3((uint32_t)base, (a.QT * a.heads_per + rows - 1) / rows), dim3(256), 0, a);
 }
 
@@ -321,7 +324,7 @@ IFR_API ifr_status ifr_paged_attention(ifr_ctx *c, const ifr_paged_cache *cache,
         const uint64_t tiles = a.search ? p->n_rows / a.QT + std::min(p->n_requests, p->n_rows) : p->n_requests;
         snprintf(name, sizeof name, "paged_rows16_%s_h%u", type, hsp);
         snprintf(merge, sizeof merge, "paged_merge16_%s_h%u", type, hsp);
-        return launch_attention(c, a, name, merge, tiles, k.dtype == IFR_F32 && hsp == 128 ? SPLIT16_F32 : SPLIT16, max_kv);
+        return launch_attention(c, a, name, merge, tiles, k.dtype == IFR_F32 && hsp == 128 ? 16 : 32, max_kv);
     }
     a.heads_per = a.G;
     a.n_sub = 1;
@@ -330,7 +333,7 @@ IFR_API ifr_status ifr_paged_attention(ifr_ctx *c, const ifr_paged_cache *cache,
     const uint64_t tiles = p->n_rows / a.QT + std::min(p->n_requests, p->n_rows);
     snprintf(name, sizeof name, "paged_tile_%s_h%u", type, hsp);
     snprintf(merge, sizeof merge, "paged_merge128_%s_h%u", type, hsp);
-    return launch_attention(c, a, name, merge, tiles, SPLIT128, max_kv);
+    return launch_attention(c, a, name, merge, tiles, 64, max_kv);
 }
 
 } // extern "C"
