@@ -36,24 +36,24 @@ uint64_t split16(uint64_t base, uint64_t n, uint32_t n_cu) {
 }
 
 // Tiles of 128 rows, n key tiles of 64. A key tile takes a workgroup 1.15 us alone on its
-// CU, two that share one 1.3 times as long; the join takes 8 us and 5 ns a workgroup for
-// its partials. The number of parts that costs least by that, of those that all have
+// CU, two that share one 1.4 times as long; the join takes 8 us and 10 ns a workgroup for
+// its partials of 128. The number of parts that costs least by that, of those that all have
 // places (`base` counts up to a tile a request too many). As chosen / another, us: 1024
 // rows of 32 heads of 128 over 4096, window 1024, 1 part 30 / 2 parts 43; 512 over 2000
 // 4 parts 41 / 1 part 54; 512 over 30000 4 parts 276 / 1 part 562; 2048 of 12 heads over
-// 4096 2 parts 95 / 1 part 117; 517 of 32 heads of 64 over 1021, f32 over f16, 4 parts 30
+// 4096 2 parts 95 / 1 part 117; 517 of 32 heads of 64 over 1021, f32 over f16, 4 parts 32
 // / 5 parts, not all with places, 34. Parts for 512 workgroups whatever n: 1024 rows over
 // none 36 (1 part: 27). At most 512 key tiles, whatever that costs: 9 requests of 1 to
 // 512 rows over 0 to 120000 keys 1497, 1024 1655, no bound 2229.
-uint64_t split128(uint64_t base, uint64_t n, uint32_t n_cu) {
+uint64_t split128(uint64_t base, uint64_t n, uint32_t hs, uint32_t n_cu) {
     uint64_t best = n;
     double least = 0.0;
     for (uint64_t parts = 1; parts <= n; parts++) {
         const uint64_t chunk = (n + parts - 1) / parts, groups = base * parts;
         if (parts > 1 && (chunk < 4 || 8 * groups > 17 * n_cu)) break;
         const double cus = (double)groups / n_cu; // workgroups a CU
-        const double step = cus <= 1.0 ? 1.0 : cus <= 2.0 ? 1.0 + 0.3 * (cus - 1.0) : 1.3 * cus / 2.0;
-        const double us = 1.15 * step * (double)chunk + (parts > 1 ? 8.0 + 0.005 * (double)groups : 0.0);
+        const double step = cus <= 1.0 ? 1.0 : cus <= 2.0 ? 1.0 + 0.4 * (cus - 1.0) : 1.4 * cus / 2.0;
+        const double us = 1.15 * step * (double)chunk + (parts > 1 ? 8.0 + 0.01 * (double)groups * hs / 128 : 0.0);
         if (parts == 1 || us < least) {
             least = us;
             best = chunk;
@@ -121,7 +121,7 @@ ifr_status launch_attention(ifr_ctx *c, PagedAttnArgs &a, const char *name, cons
     const uint64_t key_tiles = (keys + key_rows - 1) / key_rows;
     const uint64_t heads = (uint64_t)a.n_kv * a.G, row_bytes = (uint64_t)a.n_rows * heads * (a.hs + 2) * 4;
     // (key tiles of 16, of f32 rows of 128: as many keys)
-    const uint64_t chunk = key_rows == 64   ? split128(base, key_tiles, c->n_cu)
+    const uint64_t chunk = key_rows == 64   ? split128(base, key_tiles, a.hs, c->n_cu)
                            : key_rows == 32 ? split16(base, key_tiles, c->n_cu)
                                             : 2 * split16(base, (key_tiles + 1) / 2, c->n_cu);
     uint64_t splits = std::max<uint64_t>(1, std::min((key_tiles + chunk - 1) / chunk, PART_BYTES_MAX / row_bytes));
