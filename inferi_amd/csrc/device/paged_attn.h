@@ -188,7 +188,7 @@ IFR_DEV uint32_t pa_request_chunk(const PagedAttnArgs &a, uint32_t r, uint32_t r
 // The `at`-th split of all requests, the longest first (whole chunks, then the
 // requests' last parts by length): workgroups of unequal lengths, the long ones
 // started last, had left the chip half empty at the end (64 decodes of 200 to
-// 8192 rows 125 us, in the order of the requests 139).  More than 64 requests: split by split.
+// 8192 rows 123 us, in the order of the requests 139).  More than 64 requests: split by split.
 template <int KT>
 IFR_DEV bool pa_find_split(const PagedAttnArgs &a, uint32_t at, uint32_t &r, uint32_t &split) {
     const uint32_t R = a.n_requests, lane = threadIdx.x & 63;
@@ -309,13 +309,17 @@ IFR_DEV int pa_q_exponent(float mx) { return mx > 0.0f && !pa_odd(mx) ? min(14 -
 // So there is no LDS and no barrier in the loop; the waves' states are joined
 // through LDS once.  Rows whose page is no page read page 0 and are masked.
 // Bound by memory where the keys are many: 64 decodes of 200 to 8192 rows, 8 KV
-// heads of 128 in f16, 125 us, 4.7 TB/s; two of 106 K and 131 K 190 us, 5.1
+// heads of 128 in f16, 123 us, 4.8 TB/s; two of 106 K and 131 K 189 us, 5.1
 // TB/s (a large copy: 4.8).  Both need the next key tile's loads in flight over
 // the products, which is 8 waves a CU by the registers; with 12 and 43
 // registers spilled the former is 205 us.  Short calls are a chain of trips to
-// memory: one decode of 145 rows 5.5 us.  f32 caches are bound by the f32
-// products: 1629 rows over 129 of 32 heads of 128, 205 us.
-constexpr int PAD_WAVES = 4, PAD_ROWS = 16;
+// memory: one decode of 145 rows 5.5 us.
+// Chunks of f32 caches run here too, in RB = 2 blocks of 16 rows, which halve
+// what the caches behind the loads have to give (the products of one block need
+// 11 TB/s of K and V); the queries are then read from LDS.  2048 rows over 4096,
+// 32 heads of 128: 1555 us, 110 TFLOP/s (one block 1732; a library's f32 product
+// 154), 12 heads 632 (835), 32 heads of 64 825 (961).
+constexpr int PAD_WAVES = 4;
 // 16-row blocks of a key tile: two, which the f16 products' eight keys a lane
 // need; one for f32 rows of 128, whose two blocks do not fit the registers (54
 // spilled: 1191 rows over 1869 of 32 heads 379 us).
@@ -330,12 +334,12 @@ struct PaRegs {
     uint32_t v[4 * PAD_NU<HSP, T>][T == PA_S ? DV : DV / 2];
 };
 
-template <int HSP, int T>
+template <int HSP, int T, int RB>
 __device__ void pa_rows16_body(const PagedAttnArgs &a) {
-    constexpr int ES = T == PA_S ? 4 : 2, KC = PaRegs<HSP, T>::KC, DV = HSP / 16, NU = PAD_NU<HSP, T>, PAD_KT = 16 * NU;
+    constexpr int ES = T == PA_S ? 4 : 2, KC = PaRegs<HSP, T>::KC, DV = HSP / 16, NU = PAD_NU<HSP, T>, PAD_KT = 16 * NU, ROWS = 16 * RB;
     constexpr int OP = HSP + 4;
-    __shared__ __attribute__((aligned(16))) float og[PAD_WAVES][PAD_ROWS][OP];
-    __shared__ float mg[PAD_WAVES][PAD_ROWS], lg[PAD_WAVES][PAD_ROWS];
+    __shared__ __attribute__((aligned(16))) float og[PAD_WAVES][ROWS][OP];
+    __shared__ float mg[PAD_WAVES][ROWS], lg[PAD_WAVES][ROWS];
     const uint32_t tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     uint32_t b = blockIdx.x;
@@ -350,8 +354,9 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
     const uint32_t qend = a.search ? q0 + 1 : nrows, chunk = pa_request_chunk<PAD_KT>(a, r, row0, nrows, kv, last_keys);
     const uint32_t *tab = a.table + (size_t)r * a.max_pages;
     const uint32_t pm = (1u << a.lp) - 1;
-    const uint32_t qi = n / heads, hj = sub * a.heads_per + n % heads; // this lane's row
-    const uint32_t head = kvh * a.G + hj;
+    uint32_t head[RB]; // of this lane's rows n + 16 b
+#pragma unroll
+    for (int b = 0; b < RB; b++) head[b] = kvh * a.G + sub * a.heads_per + (n + 16 * b) % heads;
 
     for (; q0 < qend; q0 += a.QT) {
         const PaTile t = pa_tile(a, r, row0, nrows, kv, q0);
@@ -359,14 +364,22 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
         const uint32_t C = a.search ? pa_chunk(a, keys.n) : chunk, i0 = split * C, i1 = min(i0 + C, keys.n);
         const bool one = keys.n <= C; // (a tile without keys too: split 0 writes its zeros)
         if (i0 >= i1 && !(one && split == 0)) continue;
-        const bool row_ok = qi < t.nq;
         // a row sees the keys k <= qpos with k > qlow or k < sinks
-        const int32_t qpos = row_ok ? t.p0 + (int32_t)qi : -1, sinks = (int32_t)a.sinks;
-        const int32_t qlow = a.window ? qpos - (int32_t)a.window : -1;
-        const uint32_t gq = t.row0 + (row_ok ? qi : 0); // packed row
+        bool row_ok[RB];
+        int32_t qpos[RB], qlow[RB];
+        const int32_t sinks = (int32_t)a.sinks;
+        uint32_t gq[RB]; // packed row
+#pragma unroll
+        for (int b = 0; b < RB; b++) {
+            const uint32_t qi = (n + 16 * b) / heads;
+            row_ok[b] = qi < t.nq;
+            qpos[b] = row_ok[b] ? t.p0 + (int32_t)qi : -1;
+            qlow[b] = a.window ? qpos[b] - (int32_t)a.window : -1;
+            gq[b] = t.row0 + (row_ok[b] ? qi : 0);
+        }
 
-        float4v o[DV];
-        float m, l;
+        float4v o[RB][DV];
+        float m[RB], l[RB];
 
         auto tile_of = [&](uint32_t i) { return i < keys.ns ? i : keys.lo + i - keys.ns; };
         // page of the 16 rows from 16 * b16
@@ -431,15 +444,17 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
 
         // q: dims 32c + 8g .. of row n (f32 cache: 16c + 4g ..)
         half8v qh[T == PA_S ? 1 : KC], ql[T == PA_M ? KC : 1];
-        float4v qf[T == PA_S ? KC : 1];
+        float4v qf[T == PA_S && RB == 1 ? KC : 1];
         float rs = a.scale2; // of the row's raw scores
-        {
-            const char *qp = (const char *)a.q + ((size_t)gq * a.ld_q + (size_t)head * hs) * (T == PA_H ? 2 : 4);
+#pragma unroll
+        for (int b = 0; b < RB; b++) {
+            static_assert(RB == 1 || T == PA_S, "rows of f32 only in larger tiles");
+            const char *qp = (const char *)a.q + ((size_t)gq[b] * a.ld_q + (size_t)head[b] * hs) * (T == PA_H ? 2 : 4);
             if constexpr (T == PA_H) {
 #pragma unroll
                 for (int c = 0; c < KC; c++) {
                     const uint32_t d = 32 * c + 8 * g;
-                    const bool ok = row_ok && d < hs;
+                    const bool ok = row_ok[b] && d < hs;
                     uint4 x = *(const uint4 *)(qp + 2 * (ok ? d : 0));
                     if (!ok) x = make_uint4(0, 0, 0, 0);
                     qh[c] = __builtin_bit_cast(half8v, x);
@@ -450,7 +465,7 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
 #pragma unroll
                 for (int c = 0; c < KC; c++) {
                     const uint32_t d = 32 * c + 8 * g;
-                    const bool ok = row_ok && d < hs;
+                    const bool ok = row_ok[b] && d < hs;
                     const float4 u = *(const float4 *)(qp + 4 * (ok ? d : 0)), w = *(const float4 *)(qp + 4 * (ok ? d : 0) + 16);
                     const float y[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -475,18 +490,24 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
 #pragma unroll
                 for (int c = 0; c < KC; c++) {
                     const uint32_t d = 16 * c + 4 * g;
-                    const bool ok = row_ok && d < hs;
+                    const bool ok = row_ok[b] && d < hs;
                     const float4 x = *(const float4 *)(qp + 4 * (ok ? d : 0));
-                    qf[c] = ok ? float4v{x.x, x.y, x.z, x.w} : float4v{0, 0, 0, 0};
+                    const float4v y = ok ? float4v{x.x, x.y, x.z, x.w} : float4v{0, 0, 0, 0};
+                    if constexpr (RB == 1) qf[c] = y;
+                    else if (wave == 0) *(float4v *)&og[0][n + 16 * b][d] = y; // (two blocks' q do not fit the registers)
                 }
             }
         }
+        if constexpr (RB > 1) __syncthreads();
 
         auto clear = [&]() {
 #pragma unroll
-            for (int d = 0; d < DV; d++) o[d] = float4v{0, 0, 0, 0};
-            m = -INFINITY;
-            l = 0.0f;
+            for (int b = 0; b < RB; b++) {
+#pragma unroll
+                for (int d = 0; d < DV; d++) o[b][d] = float4v{0, 0, 0, 0};
+                m[b] = -INFINITY;
+                l[b] = 0.0f;
+            }
         };
         clear();
             for (uint32_t i = i0 + wave; i < i1; i += PAD_WAVES) {
@@ -498,25 +519,35 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                         for (int c = 0; c < KC; c++)
                             if ((T == PA_S ? 16 : 32) * c + dk >= hs) x.k[u][c] = make_uint4(0, 0, 0, 0);
                 }
-                float4v s[NU];
+                float4v s[RB][NU];
 #pragma unroll
-                for (int u = 0; u < NU; u++) {
-                    s[u] = float4v{0, 0, 0, 0};
+                for (int b = 0; b < RB; b++)
+#pragma unroll
+                    for (int u = 0; u < NU; u++) s[b][u] = float4v{0, 0, 0, 0};
+#pragma unroll
+                for (int u = 0; u < NU; u++)
 #pragma unroll
                     for (int c = 0; c < KC; c++) {
-                        if constexpr (T == PA_S) {
-                            const float4v kf = __builtin_bit_cast(float4v, x.k[u][c]);
+                        // (all reads of the queries at once would spill 74 registers)
+                        if (RB > 1 && HSP == 128 && c) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[c][e], s[u], 0, 0, 0);
-                        } else {
-                            const half8v kh = __builtin_bit_cast(half8v, x.k[u][c]);
-                            s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[c], s[u], 0, 0, 0);
-                            if constexpr (T == PA_M)
-                                s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[c], s[u], 0, 0, 0);
+                        for (int b = 0; b < RB; b++) {
+                            if constexpr (T == PA_S) {
+                                const float4v kf = __builtin_bit_cast(float4v, x.k[u][c]);
+                                float4v q;
+                                if constexpr (RB == 1) q = qf[c];
+                                else q = *(const float4v *)&og[0][n + 16 * b][16 * c + dk];
+#pragma unroll
+                                for (int e = 0; e < 4; e++)
+                                    s[b][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], q[e], s[b][u], 0, 0, 0);
+                            } else {
+                                const half8v kh = __builtin_bit_cast(half8v, x.k[u][c]);
+                                s[b][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[c], s[b][u], 0, 0, 0);
+                                if constexpr (T == PA_M)
+                                    s[b][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[c], s[b][u], 0, 0, 0);
+                            }
                         }
                     }
-                }
                 const bool bad0 = pg0 >= a.n_pages, bad1 = NU == 2 && pg1 >= a.n_pages;
                 // the next tile's K (past the last: the last again, unused)
                 load_k(kn, pn0, pn1);
@@ -524,16 +555,22 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                 const bool past = (int32_t)(k0 + PAD_KT - 1) > t.p0 || bad0 || bad1;
                 const bool behind = a.window && (int64_t)k0 <= (int64_t)t.plast - a.window;
 #pragma unroll
-                for (int u = 0; u < NU; u++) s[u] *= rs;
+                for (int b = 0; b < RB; b++)
+#pragma unroll
+                    for (int u = 0; u < NU; u++) s[b][u] *= rs;
                 if (past) {
 #pragma unroll
                     for (int u = 0; u < NU; u++) {
                         const bool gone = u ? bad1 : bad0;
-                        const int32_t first = (int32_t)(k0 + 16 * u + 4 * g);
-                        const int32_t hi = (gone ? -1 : qpos) - first, thi = (gone ? -1 : t.plast) - first;
+                        const int32_t first = (int32_t)(k0 + 16 * u + 4 * g), thi = (gone ? -1 : t.plast) - first;
+#pragma unroll
+                        for (int b = 0; b < RB; b++) {
+                            const int32_t hi = (gone ? -1 : qpos[b]) - first;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) s[b][u][e] = e <= hi ? s[b][u][e] : -INFINITY;
+                        }
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            s[u][e] = e <= hi ? s[u][e] : -INFINITY;
                             // rows of V that are on no page or past the last position have no part in the sums,
                             // whatever was left in their memory
 #pragma unroll
@@ -542,49 +579,59 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                     }
                 }
                 if (behind) {
-                    const int32_t lo = qlow - (int32_t)(k0 + 4 * g), sk = sinks - (int32_t)(k0 + 4 * g);
+                    const int32_t sk = sinks - (int32_t)(k0 + 4 * g);
+#pragma unroll
+                    for (int b = 0; b < RB; b++) {
+                        const int32_t lo = qlow[b] - (int32_t)(k0 + 4 * g);
+#pragma unroll
+                        for (int u = 0; u < NU; u++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                s[b][u][e] = (16 * u + e > lo) | (16 * u + e < sk) ? s[b][u][e] : -INFINITY;
+                    }
+                }
+                float p[RB][4 * NU];
+#pragma unroll
+                for (int b = 0; b < RB; b++) {
+                    float mt = -INFINITY;
 #pragma unroll
                     for (int u = 0; u < NU; u++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) s[u][e] = (16 * u + e > lo) | (16 * u + e < sk) ? s[u][e] : -INFINITY;
-                }
-                float mt = -INFINITY;
+                        for (int e = 0; e < 4; e++) mt = fmaxf(mt, s[b][u][e]);
+                    mt = pa_max4(mt);
+                    // the reference moves only where a row's maximum passes it by more than 8: most tiles rescale nothing
+                    if (__ballot(mt > m[b] + 8.0f)) {
+                        const float mn = fmaxf(m[b], mt), al = mn == -INFINITY ? 0.0f : softmax_exp2(m[b] - mn);
+                        m[b] = mn;
+                        l[b] *= al;
 #pragma unroll
-                for (int u = 0; u < NU; u++)
+                        for (int d = 0; d < DV; d++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) mt = fmaxf(mt, s[u][e]);
-                mt = pa_max4(mt);
-                // the reference moves only where a row's maximum passes it by more than 8: most tiles rescale nothing
-                if (__ballot(mt > m + 8.0f)) {
-                    const float mn = fmaxf(m, mt), al = mn == -INFINITY ? 0.0f : softmax_exp2(m - mn);
-                    m = mn;
-                    l *= al;
-#pragma unroll
-                    for (int d = 0; d < DV; d++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) o[d][e] *= al;
-                }
-                const float mr = m == -INFINITY ? 0.0f : m - PA_UP;
-                float p[4 * NU];
-#pragma unroll
-                for (int u = 0; u < NU; u++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        p[4 * u + e] = softmax_exp2(s[u][e] - mr);
-                        l += p[4 * u + e];
+                            for (int e = 0; e < 4; e++) o[b][d][e] *= al;
                     }
+                    const float mr = m[b] == -INFINITY ? 0.0f : m[b] - PA_UP;
+#pragma unroll
+                    for (int u = 0; u < NU; u++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            p[b][4 * u + e] = softmax_exp2(s[b][u][e] - mr);
+                            l[b] += p[b][4 * u + e];
+                        }
+                }
                 if constexpr (T == PA_S) {
 #pragma unroll
                     for (int j = 0; j < 4 * NU; j++)
 #pragma unroll
                         for (int d = 0; d < DV; d++)
-                            o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.v[j][d]), p[j], o[d], 0, 0, 0);
+#pragma unroll
+                            for (int b = 0; b < RB; b++)
+                                o[b][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.v[j][d]), p[b][j], o[b][d], 0, 0, 0);
                 } else {
                     uint32_t hi[4], lo[4];
 #pragma unroll
                     for (int j = 0; j < 8; j += 2) {
-                        if constexpr (T == PA_M) pa_split2(p[j], p[j + 1], hi[j / 2], lo[j / 2]);
-                        else hi[j / 2] = pa_pack(p[j], p[j + 1]);
+                        if constexpr (T == PA_M) pa_split2(p[0][j], p[0][j + 1], hi[j / 2], lo[j / 2]);
+                        else hi[j / 2] = pa_pack(p[0][j], p[0][j + 1]);
                     }
                     const half8v ph = __builtin_bit_cast(half8v, make_uint4(hi[0], hi[1], hi[2], hi[3]));
                     half8v pl;
@@ -599,8 +646,8 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                         w.z = __builtin_amdgcn_perm(x.v[5][d / 2], x.v[4][d / 2], sel);
                         w.w = __builtin_amdgcn_perm(x.v[7][d / 2], x.v[6][d / 2], sel);
                         const half8v vt = __builtin_bit_cast(half8v, w);
-                        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, ph, o[d], 0, 0, 0);
-                        if constexpr (T == PA_M) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, pl, o[d], 0, 0, 0);
+                        o[0][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, ph, o[0][d], 0, 0, 0);
+                        if constexpr (T == PA_M) o[0][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, pl, o[0][d], 0, 0, 0);
                     }
                 }
                 kt = kn;
@@ -611,50 +658,60 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
                 pn0 = page_of(NU * kn);
                 pn1 = page_of(NU * kn + 1);
             }
-        l = pa_sum4(l);
         // A weight of 0 times an infinity or NaN in a row of V that a query does not see is NaN (and the two parts
         // of a weight may make one of an infinity): where a sum is not finite though its weights are, the wave does
         // its keys again, one by one on the vector units, each row with those that it sees.
-        bool odd = false;
 #pragma unroll
-        for (int d = 0; d < DV; d++)
+        for (int b = 0; b < RB; b++) {
+            l[b] = pa_sum4(l[b]);
+            bool odd = false;
 #pragma unroll
-            for (int e = 0; e < 4; e++) odd |= pa_odd(o[d][e]);
-        if (__ballot(odd && row_ok && !pa_odd(l))) {
-            clear();
-            for (uint32_t i = i0 + wave; i < i1; i += PAD_WAVES)
-                for (uint32_t z = 0; z < PAD_KT; z++) {
-                    const uint32_t key = tile_of(i) * PAD_KT + z, page = page_of(key / 16);
-                    if (page >= a.n_pages || (int32_t)key > t.plast) continue;
-                    const size_t koff = (size_t)((int64_t)page * a.page_stride + (int64_t)(key & pm) * a.row_stride + (int64_t)kvh * a.head_stride);
-                    float d4 = 0.0f;
-                    for (uint32_t d = 4 * DV * g; d < min(4 * DV * (g + 1), hs); d++)
-                        d4 = fmaf(pa_at<T != PA_H>(a.q, (size_t)gq * a.ld_q + (size_t)head * hs + d), pa_at<T == PA_S>(a.key, koff + d), d4);
-                    const float s1 = pa_sum4(d4) * a.scale2;
-                    if (!((int32_t)key <= qpos & ((int32_t)key > qlow | (int32_t)key < sinks))) continue;
-                    const float mn = fmaxf(m, s1), mr = mn == -INFINITY ? 0.0f : mn;
-                    const float al = m == -INFINITY ? 0.0f : softmax_exp2(m - mr), p = softmax_exp2(s1 - mr + PA_UP);
-                    m = mn;
-                    // (0 x inf: a sum that was infinite stays so, or was NaN)
-                    l = l * al + p;
+            for (int d = 0; d < DV; d++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
+                for (int e = 0; e < 4; e++) odd |= pa_odd(o[b][d][e]);
+            if (__ballot(odd && row_ok[b] && !pa_odd(l[b]))) {
 #pragma unroll
-                        for (int d = 0; d < DV; d++) {
-                            const uint32_t dim = DV * (4 * g + e) + d;
-                            o[d][e] = (al == 0.0f ? 0.0f : o[d][e] * al) + p * pa_at<T == PA_S>(a.value, koff + min(dim, hs - 1));
-                        }
-                }
+                for (int d = 0; d < DV; d++) o[b][d] = float4v{0, 0, 0, 0};
+                m[b] = -INFINITY;
+                l[b] = 0.0f;
+                for (uint32_t i = i0 + wave; i < i1; i += PAD_WAVES)
+                    for (uint32_t z = 0; z < PAD_KT; z++) {
+                        const uint32_t key = tile_of(i) * PAD_KT + z, page = page_of(key / 16);
+                        if (page >= a.n_pages || (int32_t)key > t.plast) continue;
+                        const size_t koff = (size_t)((int64_t)page * a.page_stride + (int64_t)(key & pm) * a.row_stride + (int64_t)kvh * a.head_stride);
+                        float d4 = 0.0f;
+                        for (uint32_t d = 4 * DV * g; d < min(4 * DV * (g + 1), hs); d++)
+                            d4 = fmaf(pa_at<T != PA_H>(a.q, (size_t)gq[b] * a.ld_q + (size_t)head[b] * hs + d), pa_at<T == PA_S>(a.key, koff + d), d4);
+                        const float s1 = pa_sum4(d4) * a.scale2;
+                        if (!((int32_t)key <= qpos[b] & ((int32_t)key > qlow[b] | (int32_t)key < sinks))) continue;
+                        const float mn = fmaxf(m[b], s1), mr = mn == -INFINITY ? 0.0f : mn;
+                        const float al = m[b] == -INFINITY ? 0.0f : softmax_exp2(m[b] - mr), p = softmax_exp2(s1 - mr + PA_UP);
+                        m[b] = mn;
+                        // (0 x inf: a sum that was infinite stays so, or was NaN)
+                        l[b] = l[b] * al + p;
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+#pragma unroll
+                            for (int d = 0; d < DV; d++) {
+                                const uint32_t dim = DV * (4 * g + e) + d;
+                                o[b][d][e] = (al == 0.0f ? 0.0f : o[b][d][e] * al) + p * pa_at<T == PA_S>(a.value, koff + min(dim, hs - 1));
+                            }
+                    }
+            }
         }
 
         // the waves' states through LDS
+        if constexpr (RB > 1) __syncthreads(); // (over the queries)
 #pragma unroll
-        for (int e = 0; e < 4; e++)
+        for (int b = 0; b < RB; b++) {
 #pragma unroll
-            for (int d = 0; d < DV; d++) og[wave][n][DV * (4 * g + e) + d] = o[d][e];
-        if (g == 0) {
-            mg[wave][n] = m;
-            lg[wave][n] = l;
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int d = 0; d < DV; d++) og[wave][n + 16 * b][DV * (4 * g + e) + d] = o[b][d][e];
+            if (g == 0) {
+                mg[wave][n + 16 * b] = m[b];
+                lg[wave][n + 16 * b] = l[b];
+            }
         }
         __syncthreads();
         const uint32_t rows = t.nq * heads, quads = hs / 4;

@@ -309,9 +309,9 @@ IFR_API ifr_status ifr_paged_attention(ifr_ctx *c, const ifr_paged_cache *cache,
     // tiles' worth, us in tiles of 16 and of 128: heads of 128, 16 requests over 2000
     // keys 48.8 / 40.9, 64 over 500 44.1 / 33.2, one over 30000 50 / 56; heads of 64, 64
     // over 1000 25.6 / 26.1 and, with f32 rows, 25.8 / 30.4. Three tiles' worth: 12 rows
-    // of 4 requests over 9000 71.6 / 45.7. f32 caches (whose products run at a sixteenth
-    // of the rate and gain nothing from larger tiles) and groups of more than 64 heads
-    // (fewer than two rows of 128) always run in tiles of 16.
+    // of 4 requests over 9000 71.6 / 45.7. f32 caches, whose products run at a sixteenth of
+    // the rate, run in tiles of 16 and, with more rows, of 32 (device/paged_attn.h); groups
+    // of more than 64 heads (fewer than two rows of 128) always in tiles of 16.
     const uint32_t QT16 = std::max(16 / a.G, 1u), few = (hsp == 64 ? 2 : 1) * QT16;
     DeviceGuard dev(c->device);
     char name[64], merge[64];
@@ -319,10 +319,11 @@ IFR_API ifr_status ifr_paged_attention(ifr_ctx *c, const ifr_paged_cache *cache,
         // a group of more than 16 heads is cut into sub-groups of 16
         a.heads_per = std::min(a.G, 16u);
         a.n_sub = (a.G + 15) / 16;
-        a.QT = QT16;
         a.search = max_new > QT16;
+        const uint32_t rows = a.search && k.dtype == IFR_F32 ? 32 : 16;
+        a.QT = std::max(rows / a.heads_per, 1u);
         const uint64_t tiles = a.search ? p->n_rows / a.QT + std::min(p->n_requests, p->n_rows) : p->n_requests;
-        snprintf(name, sizeof name, "paged_rows16_%s_h%u", type, hsp);
+        snprintf(name, sizeof name, "paged_rows%u_%s_h%u", rows, type, hsp);
         snprintf(merge, sizeof merge, "paged_merge16_%s_h%u", type, hsp);
         return launch_attention(c, a, name, merge, tiles, k.dtype == IFR_F32 && hsp == 128 ? 16 : 32, max_kv);
     }

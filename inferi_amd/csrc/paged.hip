@@ -14,7 +14,7 @@ extern "C" __global__ void __launch_bounds__(PG_ROPE_THREADS) paged_rope_k(Paged
 #define PA_ROWS16(NAME, HSP, T)                                                                           \
     extern "C" __global__ void __launch_bounds__(64 * PAD_WAVES) __attribute__((amdgpu_waves_per_eu(2, 8))) \
     paged_rows16_##NAME##_h##HSP(PagedAttnArgs a) {                                                       \
-        pa_rows16_body<HSP, T>(a);                                                                        \
+        pa_rows16_body<HSP, T, 1>(a);                                                                       \
     }                                                                                                     \
     extern "C" __global__ void __launch_bounds__(256) paged_merge16_##NAME##_h##HSP(PagedAttnArgs a) {    \
         pa_merge_body<HSP, T, 16 * PAD_NU<HSP, T>, 1>(a);                                                 \
@@ -26,6 +26,12 @@ PA_ROWS16(mixed, 64, PA_M)
 PA_ROWS16(mixed, 128, PA_M)
 PA_ROWS16(f32, 64, PA_S)
 PA_ROWS16(f32, 128, PA_S)
+
+// f32 rows of chunks: two blocks of 16 rows (their merges are those of one)
+extern "C" __global__ void __launch_bounds__(64 * PAD_WAVES) __attribute__((amdgpu_waves_per_eu(2, 8)))
+paged_rows32_f32_h64(PagedAttnArgs a) { pa_rows16_body<64, PA_S, 2>(a); }
+extern "C" __global__ void __launch_bounds__(64 * PAD_WAVES) __attribute__((amdgpu_waves_per_eu(2, 8)))
+paged_rows32_f32_h128(PagedAttnArgs a) { pa_rows16_body<128, PA_S, 2>(a); }
 
 #define PA_TILE(NAME, HSP, T, WPE)                                                                             \
     extern "C" __global__ void __launch_bounds__(64 * PAT_WAVES) __attribute__((amdgpu_waves_per_eu(WPE, 8))) \
