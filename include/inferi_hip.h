@@ -335,8 +335,8 @@ IFR_API ifr_status ifr_paged_plan(ifr_ctx *ctx, const ifr_paged_plan_args *args)
  * same ld.  q and q_out may both be NULL (k and v only).  Values are rounded once, to the
  * output's or the cache's type.  A row whose position is IFR_NO_ROW is left
  * out altogether; one whose slot is not in the cache stores nothing, but its
- * q is turned.  A slot that two rows share ends with one row's values, which
- * one is not said.  q, k, v 16-byte aligned, ld_q, ld_k, ld_v
+ * q is turned.  A slot that two rows share ends with values of either, piece
+ * by piece.  q, k, v 16-byte aligned, ld_q, ld_k, ld_v
  * multiples of 4, q_out 16-byte aligned with ld_q_out a multiple of 8; fewer
  * than 2^24 rows. */
 typedef struct {

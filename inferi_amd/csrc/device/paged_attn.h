@@ -311,8 +311,8 @@ IFR_DEV int pa_q_exponent(float mx) { return mx > 0.0f && !pa_odd(mx) ? min(14 -
 // Bound by memory where the keys are many: 64 decodes of 200 to 8192 rows, 8 KV
 // heads of 128 in f16, 123 us, 4.8 TB/s; two of 106 K and 131 K 189 us, 5.1
 // TB/s (a large copy: 4.8).  Both need the next key tile's loads in flight over
-// the products, which is 8 waves a CU by the registers; with 12 and 43
-// registers spilled the former is 205 us.  Short calls are a chain of trips to
+// the products, which is 8 waves a CU by the registers; with 12 waves, and 43
+// registers spilled for them, the former is 205 us.  Short calls are a chain of trips to
 // memory: one decode of 145 rows 5.5 us.
 // Chunks of f32 caches run here too, in RB = 2 blocks of 16 rows, which halve
 // what the caches behind the loads have to give (the products of one block need
@@ -322,7 +322,7 @@ IFR_DEV int pa_q_exponent(float mx) { return mx > 0.0f && !pa_odd(mx) ? min(14 -
 constexpr int PAD_WAVES = 4;
 // 16-row blocks of a key tile: two, which the f16 products' eight keys a lane
 // need; one for f32 rows of 128, whose two blocks do not fit the registers (54
-// spilled: 1191 rows over 1869 of 32 heads 379 us).
+// spilled: 1191 rows over 1869 of 32 heads 379 us, with one 249).
 template <int HSP, int T>
 constexpr int PAD_NU = T == PA_S && HSP == 128 ? 1 : 2;
 
