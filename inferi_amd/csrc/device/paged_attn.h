@@ -114,7 +114,7 @@ IFR_DEV bool pa_pick(uint32_t mine, uint32_t left, uint32_t &src, uint32_t &befo
 // The `at`-th tile of all requests; false if there are fewer.  Up to 64
 // requests, one a lane: the tiles in the order of their last positions (by 64),
 // the farthest first, so that the workgroups with the most keys start first
-// (nine requests' chunks 513 us, in the order of the requests 567).
+// (nine requests' chunks 504 us, in the order of the requests 567).
 // More: from the last request's last tile, 64 requests a step.
 IFR_DEV bool pa_find(const PagedAttnArgs &a, uint32_t at, uint32_t &r, uint32_t &q0) {
     const uint32_t lane = threadIdx.x & 63;
@@ -765,15 +765,16 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
 // the row, so that the operand reads fall on distinct banks; V^T's operands
 // are read with the transposing LDS load (lane i of 16 gets column i of four
 // rows of 16).  Wave w brings the tile's rows 16w .. 16w + 15, which lie on
-// one page.  Bound by the matrix products, the softmax beside them and power:
-// 5720 rows of nine requests over 306 to 8000, 32 heads of 128, 492 GFLOP in
-// 513 us, 0.96 PFLOP/s with the matrix pipes 42-47% busy (a library's f16
-// product of 8192^3: 1.14).  Scores one key tile ahead of the softmax took fewer
-// cycles but as long (the clock fell from 2.0 to 1.7 GHz); one buffer of V and
-// three workgroups a CU 592 us.  Of f32 rows, whose products are done twice and
-// whose weights are split on the vector units, 517 over 1021, 32 heads of 64: 22
-// us, and the merge 8.
-constexpr int PAT_WAVES = 4, PAT_ROWS = 32 * PAT_WAVES, PAT_KT = 64;
+// one page.  Bound by the operand reads from LDS (128 KB a key tile and
+// workgroup, 1024 cycles, as long as its products), the softmax beside them
+// and power: 5720 rows of nine requests over 306 to 8000, 32 heads of 128, 492
+// GFLOP in 504 us, 0.98 PFLOP/s with the matrix pipes 42-47% busy (a library's
+// f16 product of 8192^3: 1.14).  Scores one key tile ahead of the softmax, in
+// three forms, measured 1 to 4% slower (the clock falls from 2.0 to 1.7 GHz);
+// one buffer of V and three workgroups a CU 592 us.  f32 rows, whose products
+// are done twice and whose weights are split on the vector units: 517 over 1021,
+// 32 heads of 64, 23 us, and the merge 8.
+constexpr int PAT_WAVES = 4, PAT_KT = 64;
 
 template <int HSP, int T>
 __device__ void pa_tile_body(const PagedAttnArgs &a) {

@@ -402,6 +402,16 @@ def test_unequal_decodes_past_the_bound(ctx, kind, max_kv):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [1, 3, 33, 64, 130])
+def test_equal_decodes(ctx, kind, n):
+    """Decodes of the same length, around the lengths where they are split, with requests that have no rows between."""
+    rng = np.random.default_rng(22)
+    for c in (510, 511, 512, 544, 1023, 1024, 1100):
+        lens = [(7, 0) if i % 13 == 5 else (c, 1) for i in range(n)]
+        check(*attn_case(ctx, rng, kind, 4, 2, 64, 32, lens))
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("requests", [1, 5, 66])
 def test_windows_with_more_rows_than_the_bound(ctx, kind, requests):
     """Rows past max_new under a window of some whole chunks of keys: a request's earlier tiles reach over more key
