@@ -111,12 +111,12 @@ IFR_DEV bool pa_pick(uint32_t mine, uint32_t left, uint32_t &src, uint32_t &befo
     before = __builtin_amdgcn_readlane(sum - mine, src);
     return true;
 }
-// The `at`-th tile of all requests; false if there are fewer.  Up to 64
-// requests, one a lane: the tiles in the order of their last positions (by 64),
+// The `at`-th tile of all requests; false if there are fewer.  Sorted and up to
+// 64 requests, one a lane: the tiles in the order of their last positions (by 64),
 // the farthest first, so that the workgroups with the most keys start first
 // (nine requests' chunks 504 us, in the order of the requests 567).
-// More: from the last request's last tile, 64 requests a step.
-IFR_DEV bool pa_find(const PagedAttnArgs &a, uint32_t at, uint32_t &r, uint32_t &q0) {
+// Else from the last request's last tile, 64 requests a step (16 of 4 rows over 300 6.6 us, sorted 7.1).
+IFR_DEV bool pa_find(const PagedAttnArgs &a, bool sorted, uint32_t at, uint32_t &r, uint32_t &q0) {
     const uint32_t lane = threadIdx.x & 63;
     uint32_t src = 0, before = 0;
     if (a.n_requests == 1) {
@@ -127,7 +127,7 @@ IFR_DEV bool pa_find(const PagedAttnArgs &a, uint32_t at, uint32_t &r, uint32_t 
         q0 = (nt - 1 - at) * a.QT;
         return at < nt;
     }
-    if (a.n_requests <= 64) {
+    if (sorted) {
         uint32_t row0, n = 0, kv = 0, nt = 0;
         if (lane < a.n_requests) {
             pa_request(a, lane, row0, n, kv);
@@ -352,7 +352,7 @@ __device__ void pa_rows16_body(const PagedAttnArgs &a) {
     b /= a.n_sub;
     const uint32_t hs = a.hs, heads = min(a.heads_per, a.G - sub * a.heads_per);
     uint32_t r, q0 = 0, split = blockIdx.y, row0, nrows, kv, last_keys;
-    if (a.search ? !pa_find(a, b, r, q0) : !pa_find_split<PAD_KT>(a, b, r, split)) return;
+    if (a.search ? !pa_find(a, a.sorted, b, r, q0) : !pa_find_split<PAD_KT>(a, b, r, split)) return;
     pa_request_uniform(a, r, row0, nrows, kv);
     const uint32_t qend = a.search ? q0 + 1 : nrows, chunk = pa_request_chunk<PAD_KT>(a, r, row0, nrows, kv, last_keys);
     const uint32_t *tab = a.table + (size_t)r * a.max_pages;
@@ -792,7 +792,7 @@ __device__ void pa_tile_body(const PagedAttnArgs &a) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t kvh = blockIdx.x % a.n_kv, split = blockIdx.y;
     uint32_t r, q0, row0, nrows, kv;
-    if (!pa_find(a, blockIdx.x / a.n_kv, r, q0)) return;
+    if (!pa_find(a, a.sorted, blockIdx.x / a.n_kv, r, q0)) return;
     pa_request_uniform(a, r, row0, nrows, kv);
     const PaTile t = pa_tile(a, r, row0, nrows, kv, q0);
     const PaKeys keys = pa_keys<PAT_KT>(a, t);
@@ -1126,7 +1126,7 @@ __device__ void pa_merge_body(const PagedAttnArgs &a) {
     b /= a.n_sub;
     const uint32_t hs = a.hs, heads = min(a.heads_per, a.G - sub * a.heads_per);
     uint32_t r = b, q0 = 0, row0, nrows, kv;
-    if (a.search && !pa_find(a, b, r, q0)) return;
+    if (a.search && !pa_find(a, false, b, r, q0)) return;
     pa_request_uniform(a, r, row0, nrows, kv);
     uint32_t last_keys;
     const uint32_t qend = a.search ? q0 + 1 : nrows, chunk = pa_request_chunk<KT>(a, r, row0, nrows, kv, last_keys);

@@ -133,7 +133,7 @@ ifr_status launch_attention(ifr_ctx *c, PagedAttnArgs &a, const char *name, cons
         a.part_o = (float *)c->scratch;
         a.part_ml = a.part_o + (uint64_t)a.n_rows * heads * splits * a.hs;
     }
-    a.sorted = !a.search && a.n_requests > 1 && a.n_requests <= 64 && base * splits > (uint32_t)c->n_cu;
+    a.sorted = a.n_requests > 1 && a.n_requests <= 64 && base * splits > (uint32_t)c->n_cu;
     // (without a search a workgroup finds its split with its request)
     const dim3 grid = a.search ? dim3((uint32_t)base, a.n_splits) : dim3((uint32_t)(base * splits));
     ifr_status st = c->launch(name, grid, dim3(256), 0, a);

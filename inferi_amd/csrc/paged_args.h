@@ -43,7 +43,7 @@ struct PagedAttnArgs {
     uint32_t n_splits, chunk; // workgroups that share a tile's keys, at most; key tiles of each, at least
     uint32_t QT, heads_per, n_sub; // queries of a tile; heads of a sub-group; sub-groups of a KV head's heads
     uint32_t search; // a workgroup finds its tile among all requests' (else: tile = request)
-    uint32_t sorted; // the longest splits of up to 64 requests first (without a search)
+    uint32_t sorted; // the longest tiles or splits of up to 64 requests first
     float scale2;                  // scale x log2(e)
 };
 
