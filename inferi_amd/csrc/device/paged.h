@@ -71,15 +71,15 @@ IFR_DEV void last_at_most_of(const uint32_t *a, uint32_t n, uint32_t x0, uint32_
 }
 
 // Position and slot of row `row`, which is request r's (rows from `start` to
-// `end`; kv rows of the cache after the step, 0: not granted).  page_of(i): the
-// page with the request's rows from i << lp.
+// `end`; kv rows of the cache after the step, 0: not granted).  page_of(i, first):
+// the page with the request's rows from i << lp (first: this row is its first).
 template <class F>
 IFR_DEV void paged_row(const PagedPlanArgs &a, uint32_t row, uint32_t start, uint32_t end, uint32_t kv, F page_of) {
     uint32_t pos = PG_NO_ROW;
     uint64_t slot = ~0ull;
     if (kv && row < end) {
         pos = kv - (end - start) + (row - start);
-        const uint32_t page = page_of(pos >> a.lp);
+        const uint32_t page = page_of(pos >> a.lp, !(pos & ((1u << a.lp) - 1)));
         if (page < a.n_pages) slot = ((uint64_t)page << a.lp) + (pos & ((1u << a.lp) - 1));
     }
     a.positions[row] = pos;
@@ -93,7 +93,8 @@ IFR_DEV void paged_row(const PagedPlanArgs &a, uint32_t row, uint32_t start, uin
 // latency of its chain: lengths, a scan, the popped pages with the pages of the
 // rows.  The rows take their pages from where they come from (the request's
 // last page, or the free list), not from the table entries written beside them.
-// 32 decodes 4.1 us, 1021 requests 13 (a launch that does nothing: 3.3).
+// 32 decodes 4.1 us, 1021 requests of which a tenth are released 10 (a launch that
+// does nothing: 3.3).
 __device__ inline void paged_plan_body(const PagedPlanArgs &a) {
     __shared__ uint32_t part[32], s_fresh;
     __shared__ uint32_t s_start[PG_PLAN_THREADS + 1], s_off[PG_PLAN_THREADS], s_held[PG_PLAN_THREADS], s_kv[PG_PLAN_THREADS];
@@ -190,12 +191,15 @@ __device__ inline void paged_plan_body(const PagedPlanArgs &a) {
         if (ok && need) atomicMax(&s_fresh, off + need);
         __syncthreads();
         const uint32_t fresh = max(s_fresh, taken);
+        // where the rows are another launch's, their new pages' entries are too, from where each request's pages begin
+        if (!a.rows_here && in) a.pops[r] = off;
         // the round's new table entries: popped page i is request j's, the last one whose pages begin at or before
         // i (one without new pages shares its place with the next)
         auto entry = [&](uint32_t i, uint32_t j) {
             a.table[(size_t)(base + j) * a.max_pages + s_held[j] + (i - s_off[j])] = a.free_pages[top - 1 - i];
         };
-        if (fresh - taken <= T) {
+        if (!a.rows_here) {
+        } else if (fresh - taken <= T) {
             if (taken + tid < fresh) entry(taken + tid, last_at_most(s_off, nr, taken + tid));
         } else {
             for (uint32_t i = taken + 4 * tid; i < fresh; i += 4 * T) {
@@ -211,7 +215,7 @@ __device__ inline void paged_plan_body(const PagedPlanArgs &a) {
 #pragma unroll 2
             for (uint32_t row = first + tid; row < last; row += T) {
                 const uint32_t j = last_at_most(s_start, nr, row);
-                paged_row(a, row, s_start[j], s_start[j + 1], s_kv[j], [&](uint32_t i) {
+                paged_row(a, row, s_start[j], s_start[j + 1], s_kv[j], [&](uint32_t i, bool) {
                     return i < s_held[j] ? a.table[(size_t)(base + j) * a.max_pages + i]
                                          : a.free_pages[top - 1 - (s_off[j] + i - s_held[j])];
                 });
@@ -223,21 +227,23 @@ __device__ inline void paged_plan_body(const PagedPlanArgs &a) {
         __syncthreads();
     }
     if (!a.n_requests) // no request has any of the rows
-        for (uint32_t row = tid; row < a.n_rows; row += T) paged_row(a, row, 0, 0, 0, [](uint32_t) { return 0u; });
+        for (uint32_t row = tid; row < a.n_rows; row += T) paged_row(a, row, 0, 0, 0, [](uint32_t, bool) { return 0u; });
     if (tid == 0) {
         a.row_start[a.n_requests] = min(rows0, a.n_rows);
         *a.free_count_out = top - taken;
+        if (!a.rows_here) a.pops[a.n_requests] = top;
     }
 }
 
-// The rows of a large step, 256 threads each with rows of its own.  A
-// workgroup finds its first row's request by a 256-way search of row_start,
-// and its rows' among the next 1024 requests' starts in LDS: 58885 rows of 1021
-// requests 5 us.
+// The rows of a large step, 256 threads each with rows of their own, and the
+// table entries of their new pages (every new page has a new row that is its
+// first).  A workgroup finds its first row's request by a 256-way search of
+// row_start, and its rows' among the next 1024 requests' starts in LDS: 58885
+// rows of 1021 requests 5 us.
 constexpr uint32_t PG_ROWS_PER = 512, PG_ROWS_WIN = 1024;
 
 __device__ inline void paged_rows_body(const PagedPlanArgs &a) {
-    __shared__ uint32_t s_start[PG_ROWS_WIN + 1], s_kv[PG_ROWS_WIN], s_n;
+    __shared__ uint32_t s_start[PG_ROWS_WIN + 1], s_kv[PG_ROWS_WIN], s_pops[PG_ROWS_WIN], s_n;
     const uint32_t tid = threadIdx.x, row0 = blockIdx.x * PG_ROWS_PER;
     // the last request that starts at or before row0 (requests without rows
     // share their start with the next: the last one of them has row0)
@@ -258,18 +264,28 @@ __device__ inline void paged_rows_body(const PagedPlanArgs &a) {
     for (uint32_t i = tid; i < nr; i += 256) {
         s_start[i] = a.row_start[r0 + i];
         s_kv[i] = a.kv_len[r0 + i];
+        s_pops[i] = a.pops[r0 + i];
     }
     if (tid == 0) s_start[nr] = a.row_start[r0 + nr];
     __syncthreads();
+    const uint32_t top = a.pops[a.n_requests], pm = (1u << a.lp) - 1;
+    auto fill = [&](uint32_t row, uint32_t r, uint32_t start, uint32_t end, uint32_t kv, uint32_t pops) {
+        const uint32_t held = (kv - (end - start) + pm) >> a.lp; // (of a granted request)
+        paged_row(a, row, start, end, kv, [&](uint32_t i, bool first) {
+            uint32_t *entry = a.table + (size_t)r * a.max_pages + i;
+            if (i < held) return *entry;
+            const uint32_t page = a.free_pages[top - 1 - (pops + i - held)];
+            if (first) *entry = page;
+            return page;
+        });
+    };
     for (uint32_t row = row0 + tid; row < min(row0 + PG_ROWS_PER, a.n_rows); row += 256) {
         if (row < s_start[nr] || r0 + nr == a.n_requests) {
             const uint32_t j = last_at_most(s_start, nr, row);
-            paged_row(a, row, s_start[j], s_start[j + 1], s_kv[j],
-                      [&](uint32_t i) { return a.table[(size_t)(r0 + j) * a.max_pages + i]; });
+            fill(row, r0 + j, s_start[j], s_start[j + 1], s_kv[j], s_pops[j]);
         } else { // more requests than the window between this row and the workgroup's first
             const uint32_t r = last_at_most(a.row_start, a.n_requests, row);
-            paged_row(a, row, a.row_start[r], a.row_start[r + 1], a.kv_len[r],
-                      [&](uint32_t i) { return a.table[(size_t)r * a.max_pages + i]; });
+            fill(row, r, a.row_start[r], a.row_start[r + 1], a.kv_len[r], a.pops[r]);
         }
     }
 }

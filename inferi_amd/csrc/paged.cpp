@@ -180,8 +180,12 @@ IFR_API ifr_status ifr_paged_plan(ifr_ctx *c, const ifr_paged_plan_args *p) {
     a.n_pages = p->n_pages;
     a.lp = log2_of(p->page_size);
     a.max_pages = p->max_pages;
-    // (2048 rows by the plan's workgroup 4.9 us, by a second launch 7.4; 3074 6.0 and 7.5; 11274 11.9 and 11.3)
-    a.rows_here = p->n_rows <= 8192 || !p->n_requests;
+    // (us by the plan's workgroup / by a second launch: 2048 rows 4.8 / 6.9, 3074 6.0 / 7.0, 4611 6.9 / 7.0, 7170 8.6 / 7.2)
+    a.rows_here = p->n_rows <= 4096 || !p->n_requests;
+    if (!a.rows_here) {
+        if (ifr_status st = c->ensure_scratch(((size_t)p->n_requests + 1) * 4)) return st;
+        a.pops = (uint32_t *)c->scratch;
+    }
     const uint32_t widest = std::max(p->n_requests, a.rows_here ? p->n_rows : 0u);
     const uint32_t threads = widest <= 64 ? 64 : widest <= 256 ? 256 : PG_PLAN_THREADS;
     ifr_status st = c->launch("paged_plan_k", dim3(1), dim3(threads), 0, a);

@@ -17,7 +17,8 @@ struct PagedPlanArgs {
     uint32_t *free_count_out, *table, *ctx_len_out, *row_start, *kv_len, *positions;
     uint64_t *slots;
     uint32_t n_requests, n_rows, n_pages, lp, max_pages; // page size 1 << lp
-    uint32_t rows_here; // the plan kernel fills the rows itself
+    uint32_t rows_here; // the plan kernel fills the rows and the table itself
+    uint32_t *pops;     // else: where each request's popped pages begin; after the last, the stack's height
 };
 
 struct PagedRopeArgs {

@@ -77,6 +77,16 @@ def test_plan_rows_short_and_spare(ctx, n, rows):
         np.testing.assert_array_equal(got[k], ref[k], err_msg=k)
 
 
+@pytest.mark.parametrize("n,page,spare,release", [(40, 16, 0, 0.0), (300, 64, -40, 0.1), (1100, 16, -900, 0.05), (2100, 32, 7, 0.2)])
+def test_plan_of_many_rows(ctx, n, page, spare, release):
+    """Steps whose rows are a launch of their own, some with too few pages for the last requests."""
+    case = _plan_case(np.random.default_rng(n), n, page, 60, spare, release, max_new=600)
+    assert case[-1] > 8192
+    got, ref = run_plan(ctx, *case), plan_ref(*case)
+    for k in ref:
+        np.testing.assert_array_equal(got[k], ref[k], err_msg=k)
+
+
 def test_plan_long_prompts_and_no_requests(ctx):
     page, most = 16, 4096
     free = np.random.default_rng(5).permutation(5000).astype(np.uint32)
